@@ -47,6 +47,7 @@ extern "C" {
 #define DSMOE_DTYPE_F32 0
 #define DSMOE_DTYPE_BF16 1
 #define DSMOE_DTYPE_E4M3 2
+#define DSMOE_DTYPE_I8 3
 
 /* Largest decode batch of dsmoe_moe_decode (tokens per call). */
 #define DSMOE_MAX_DECODE_TOKENS 64
@@ -126,6 +127,61 @@ DSMOE_API int dsmoe_fp4_gemm(const void* a, int a_dtype, const float* a_s, long 
  * `act_quant` (dsv41/ref/kernel.py:44-55). x: [M, K] in x_dtype (F32 or BF16). */
 DSMOE_API int dsmoe_act_quant(const void* x, int x_dtype, long long M, long long K, int block, int pow2,
                     uint8_t* q, float* s, void* stream);
+
+/* ---- 8-bit operators around the expert products ------------------------------------------- */
+
+/* r = x + residual rounded to dtype (residual NULL: r = x), v = r / sqrt(mean(r^2) + eps) * weight per
+ * row, v quantized: q_dtype DSMOE_DTYPE_E4M3 as in dsmoe_act_quant (one scale per 128 values, hidden a
+ * multiple of 128, pow2 as there, s [rows, hidden / 128]), DSMOE_DTYPE_I8 with one scale per row,
+ * s = max(amax, 1e-4) / 127, q = rint(v / s), s [rows]. residual_out (r; may be residual or x itself)
+ * and normed (v rounded to dtype) may be NULL. dtype F32 or BF16, weight [hidden] F32 or BF16, hidden
+ * <= 16384. A row (E4M3: a block) with an infinity or NaN gets the scale NaN. E4M3 wants 16-byte
+ * aligned pointers. Feeds dsmoe_fp8_gemm / dsmoe_int8_gemm. */
+DSMOE_API int dsmoe_rms_norm_quant(const void* x, int dtype, const void* residual, const void* weight, int w_dtype,
+                                   long long rows, long long hidden, float eps, int q_dtype, int pow2, void* q, float* s,
+                                   void* residual_out, void* normed, void* stream);
+
+/* v = silu(min(g, limit)) * clamp(u, -limit, limit) * row_weight[row] (NULL: 1) for gu [rows, 2 inter] =
+ * g | u, quantized as above: the expert FFN's activation (dsv41/tt/moe.py:133-139) between two 8-bit
+ * products. */
+DSMOE_API int dsmoe_swiglu_quant(const void* gu, int dtype, const float* row_weight, long long rows, long long inter,
+                                 float limit, int q_dtype, int pow2, void* q, float* s, void* stream);
+
+/* out[M, N] = (a b^T) a_s[m] b_s[n] for int8 a [M, K], b [N, K]: an exact int32 sum, converted to fp32,
+ * multiplied by the scales, rounded to out_dtype (F32 or BF16). K a multiple of 16, at most 131071;
+ * a, b 16-byte aligned. On the 5th-generation tensor cores (kind::i8). Uses no workspace. */
+DSMOE_API int dsmoe_int8_gemm(const int8_t* a, const float* a_s, long long M, long long K, const int8_t* b,
+                              const float* b_s, long long N, void* out, int out_dtype, void* stream);
+
+/* The experts' products over rows sorted by expert: rows offsets[e]..offsets[e + 1] - 1 of a [M, K] times
+ * b[e] [N, K] with scales b_s[e] [N]; offsets [n_experts + 1] int32 on the device (dsmoe_sort_tokens),
+ * n_experts <= 1024. Rows at and behind offsets[n_experts] of out are zero. Offsets that do not rise from 0
+ * to at most M give NaN throughout. */
+DSMOE_API int dsmoe_int8_grouped_gemm(const int8_t* a, const float* a_s, long long M, long long K, const int8_t* b,
+                                      const float* b_s, int n_experts, long long N, const int* offsets, void* out,
+                                      int out_dtype, void* stream);
+
+/* Choices sorted by (expert, token, choice): idx [P, k] int64 -> pos [P, k] int32 (row of each choice, -1
+ * where idx is outside 0..n_experts-1: dropped), src [P k] int32 (choice t k + j of each row, -1 behind the
+ * last), offsets [n_experts + 1] int32 (first row of each expert). k <= 64, n_experts <= 1024, P k < 2^30. */
+DSMOE_API int dsmoe_sort_tokens(const int64_t* idx, long long P, int k, int n_experts, int* pos, int* src, int* offsets,
+                                void* stream);
+
+/* xs[pos[t, j]] = x[t] for rows of row_bytes bytes of any type (and ss[pos[t, j]] = s[t] where s is not
+ * NULL); rows of xs behind offsets[n_experts] are zero. xs has P k rows. */
+DSMOE_API int dsmoe_dispatch_rows(const void* x, const float* s, const int* pos, const int* offsets, int n_experts,
+                                  long long P, int k, long long row_bytes, void* xs, float* ss, void* stream);
+
+/* y[t] = sum_j wt[t, j] ys[pos[t, j]] over the choices that were not dropped, in fp32, in order of j, rounded
+ * once; dtype F32 or BF16. wt NULL: all ones, which is the gradient of dsmoe_dispatch_rows. */
+DSMOE_API int dsmoe_combine_rows(const void* ys, int dtype, const int* pos, const float* wt, long long P, int k,
+                                 long long width, void* y, void* stream);
+
+/* Gradients of dsmoe_combine_rows: dys[pos[t, j]] = wt[t, j] dy[t] (rows behind the last: zero) and
+ * dwt[t, j] = <dy[t], ys[pos[t, j]]> (dropped: 0). dys or dwt may be NULL; ys only with dwt NULL. */
+DSMOE_API int dsmoe_combine_grad(const void* dy, const void* ys, int dtype, const int* pos, const float* wt,
+                                 const int* offsets, int n_experts, long long P, int k, long long width, void* dys,
+                                 float* dwt, void* stream);
 
 /* ---- expert store (one-time repack; replaces the host ExpertStore / tile packer) ---------- */
 

@@ -16,7 +16,7 @@ OK, ERR_ARG, ERR_ALIGN, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT, ERR_UNSUPPORTED = 
 FMT_FP8, FMT_FP4 = 0, 1
 LAYOUT_FRAG, LAYOUT_TC = 0, 1
 SCORE_SIGMOID, SCORE_SQRTSOFTPLUS = 0, 1
-DTYPE_F32, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2
+DTYPE_F32, DTYPE_BF16, DTYPE_E4M3, DTYPE_I8 = 0, 1, 2, 3
 MAX_DECODE_TOKENS = 64
 COMM_HANDLE_BYTES = 64
 SLOT_TOKENS = 8
@@ -52,6 +52,14 @@ _SIGS = {
     "dsmoe_fp8_gemm": ([_P, _I, _P, _LL, _LL, _P, _P, _LL, _P, _I, _P], _I),
     "dsmoe_fp4_gemm": ([_P, _I, _P, _LL, _LL, _P, _P, _LL, _P, _I, _P], _I),
     "dsmoe_act_quant": ([_P, _I, _LL, _LL, _I, _I, _P, _P, _P], _I),
+    "dsmoe_rms_norm_quant": ([_P, _I, _P, _P, _I, _LL, _LL, _F, _I, _I, _P, _P, _P, _P, _P], _I),
+    "dsmoe_swiglu_quant": ([_P, _I, _P, _LL, _LL, _F, _I, _I, _P, _P, _P], _I),
+    "dsmoe_int8_gemm": ([_P, _P, _LL, _LL, _P, _P, _LL, _P, _I, _P], _I),
+    "dsmoe_int8_grouped_gemm": ([_P, _P, _LL, _LL, _P, _P, _I, _LL, _P, _P, _I, _P], _I),
+    "dsmoe_sort_tokens": ([_P, _LL, _I, _I, _P, _P, _P, _P], _I),
+    "dsmoe_dispatch_rows": ([_P, _P, _P, _P, _I, _LL, _I, _LL, _P, _P, _P], _I),
+    "dsmoe_combine_rows": ([_P, _I, _P, _P, _LL, _I, _LL, _P, _P], _I),
+    "dsmoe_combine_grad": ([_P, _P, _I, _P, _P, _P, _I, _LL, _I, _LL, _P, _P, _P], _I),
     "dsmoe_store_expert_bytes": ([_I, _I, _I, ctypes.POINTER(_LL), ctypes.POINTER(_LL)], _I),
     "dsmoe_store_pack_expert": ([_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P], _I),
     "dsmoe_store_unpack_expert": ([_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P], _I),

@@ -17,8 +17,9 @@ from typing import Optional
 import torch
 
 from . import _lib as L
+from . import ops
 from .store import ExpertStore
-from .synth import ExpertWeights, RouterWeights
+from .synth import ExpertWeights, RouterWeights, quant_int8_channel
 
 LIMIT = 10.0  # SwiGLU clamp (dsv41/tt/moe.py:15)
 
@@ -337,5 +338,59 @@ class Expert:
         if weight is not None:
             h = h * weight.float().view(-1, 1)
         return self._lin(h, self.ew.w2, self.ew.s2, hidden)
+
+    __call__ = forward
+
+
+class Int8Experts:
+    """The routed experts in 8-bit integers (one scale per output channel and per token), for any routing.
+
+    y[t] = sum_j wt[t, j] * w2( silu(min(w1 x, 10)) * clamp(w3 x, -10, 10) ) over the experts idx[t, j]:
+    the operators of ``ops`` in a row -- tokens sorted by expert, the w1|w3 products of every expert in
+    one launch, the activation to int8, the w2 products, and the weighted sum back (dsv41/tt/moe.py:133-139,
+    182-200, with the routing weight applied after w2).
+    """
+
+    def __init__(self, hidden: int, inter: int, n_experts: int, device=None):
+        if hidden % 16 or inter % 16:
+            raise ValueError(f"hidden {hidden} and inter {inter} must be multiples of 16")
+        self.hidden, self.inter, self.n_experts = hidden, inter, n_experts
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.w13 = torch.zeros((n_experts, 2 * inter, hidden), dtype=torch.int8, device=self.device)
+        self.s13 = torch.zeros((n_experts, 2 * inter), dtype=torch.float32, device=self.device)
+        self.w2 = torch.zeros((n_experts, hidden, inter), dtype=torch.int8, device=self.device)
+        self.s2 = torch.zeros((n_experts, hidden), dtype=torch.float32, device=self.device)
+
+    def load_expert(self, e: int, ew: ExpertWeights) -> None:
+        """Requantize expert ``e`` from its checkpoint format (FP8 or FP4) to int8, on the GPU."""
+        if not 0 <= e < self.n_experts:
+            raise IndexError(e)
+        i, h = self.inter, self.hidden
+        for q, s, n, k, dst, scale in ((ew.w1, ew.s1, i, h, self.w13[e, :i], self.s13[e, :i]),
+                                       (ew.w3, ew.s3, i, h, self.w13[e, i:], self.s13[e, i:]),
+                                       (ew.w2, ew.s2, h, i, self.w2[e], self.s2[e])):
+            q, s = q.to(self.device).contiguous(), s.to(self.device).contiguous()
+            if tuple(q.shape) != (n, k if ew.fmt == "fp8" else k // 2):
+                raise ValueError(f"expert weights {tuple(q.shape)} do not match hidden {h} / inter {i} ({ew.fmt})")
+            w = torch.empty((n, k), dtype=torch.float32, device=self.device)
+            with torch.cuda.device(self.device):
+                if ew.fmt == "fp8":
+                    L.call("dsmoe_fp8_block_dequant", L.ptr(q), L.ptr(s), n, k, 128, L.ptr(w), L.DTYPE_F32, L.stream_of(w))
+                else:
+                    L.call("dsmoe_fp4_dequant", L.ptr(q), L.ptr(s), n, k, L.ptr(w), L.DTYPE_F32, L.stream_of(w))
+            codes, scales = quant_int8_channel(w)
+            dst.copy_(codes)
+            scale.copy_(scales)
+
+    def forward(self, x: torch.Tensor, x_s: torch.Tensor, idx: torch.Tensor, wt: torch.Tensor,
+                out_dtype=torch.bfloat16) -> torch.Tensor:
+        """x [tokens, hidden] int8 with x_s [tokens] (``rms_norm_quant(..., fmt="int8")``), idx [tokens, k] int64
+        and wt [tokens, k] fp32 (``MoE.route``) -> y [tokens, hidden]. Choices of -1 are left out."""
+        order = ops.sort_tokens(idx, self.n_experts)
+        xs, ss = ops.dispatch_tokens(x, order, x_s)
+        gu = ops.int8_grouped_gemm(xs, ss, self.w13, self.s13, order.offsets, out_dtype=torch.bfloat16)
+        h, hs = ops.swiglu_quant(gu, limit=LIMIT, fmt="int8")
+        ys = ops.int8_grouped_gemm(h, hs, self.w2, self.s2, order.offsets, out_dtype=out_dtype)
+        return ops.combine_tokens(ys, order, wt)
 
     __call__ = forward

@@ -55,6 +55,12 @@ def quant_fp4_e8m0(w: torch.Tensor, group: int = 32):
     return packed, e8
 
 
+def quant_int8_channel(w: torch.Tensor):
+    """fp32 [N, K] -> (int8 [N, K], fp32 scales [N], one per output channel: channel max / 127)."""
+    s = w.abs().amax(dim=1).clamp(min=1e-30) / 127.0
+    return (w / s.unsqueeze(1)).round().clamp(-127.0, 127.0).to(torch.int8), s
+
+
 @dataclass
 class ExpertWeights:
     """One expert in the checkpoint layout: w1/w3 [I, H], w2 [H, I] (quantized), and their scales."""

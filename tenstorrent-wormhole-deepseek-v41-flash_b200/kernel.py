@@ -4,7 +4,8 @@
 the same way and the model's ``import kernel`` gets B200 kernels.
 
 Same names, signatures and return dtypes as the shim (dsv41/ref/kernel.py:44, 58, 91, 105, 110),
-plus ``weight_dequant`` (the FP8 block dequant entry point of DeepSeek's kernel module).
+plus ``weight_dequant`` (the FP8 block dequant entry point of DeepSeek's kernel module) and, from
+``dsmoe.ops``, ``rms_norm_quant``, ``swiglu_quant`` and ``int8_gemm``, which quantize always.
 ``DSV41_FAKEQUANT`` has the shim's meaning and default (dsv41/ref/kernel.py:36-41): "0" keeps
 activations exact, anything else fake-quantizes linear inputs to e4m3 per 128.
 
@@ -16,6 +17,7 @@ import os as _os
 import torch
 
 from dsmoe import _lib as _L
+from dsmoe.ops import int8_gemm, rms_norm_quant, swiglu_quant  # noqa: F401  (beside fp8_gemm, act_quant)
 
 FAKEQUANT = _os.environ.get("DSV41_FAKEQUANT", "1") != "0"
 

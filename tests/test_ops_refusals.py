@@ -1,0 +1,110 @@
+"""The 8-bit operators' C entry points refuse bad calls before they touch the device (no GPU here), and
+their Python surface takes CUDA tensors only."""
+import pytest
+import torch
+
+A = 4096  # an aligned address that no call may reach
+
+
+def _code(name, *args):
+    from dsmoe import _lib as L
+    return getattr(L.lib, name)(*args)
+
+
+NORM = dict(x=A, dtype=1, residual=2 * A, weight=3 * A, w_dtype=0, rows=4, hidden=256, eps=1e-6, q_dtype=2, pow2=0, q=A * 4,
+            s=A * 8, residual_out=A * 12, normed=None, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(x=None), -1), (dict(weight=None), -1), (dict(q=None), -1), (dict(s=None), -1), (dict(dtype=2), -1),
+    (dict(w_dtype=3), -1), (dict(q_dtype=1), -1), (dict(rows=0), -1), (dict(rows=-1), -1), (dict(rows=1 << 31), -1),
+    (dict(hidden=0), -1), (dict(hidden=130), -1), (dict(hidden=16512), -1), (dict(residual=None), -1),
+    (dict(q_dtype=3, pow2=1), -1), (dict(x=A + 2), -2), (dict(x=A + 1, q_dtype=3), -2), (dict(s=A * 8 + 2), -2),
+    (dict(weight=3 * A + 2), -2), (dict(residual_out=2 * A + 64), -1), (dict(normed=A), -1), (dict(normed=A * 12), -1),
+    (dict(q=A), -1), (dict(normed=2 * A + 512), -1)])
+def test_rms_norm_quant_refuses(change, code):
+    assert _code("dsmoe_rms_norm_quant", *{**NORM, **change}.values()) == code
+
+
+SWIGLU = dict(gu=A, dtype=1, row_weight=None, rows=4, inter=256, limit=10.0, q_dtype=2, pow2=0, q=A * 4, s=A * 8, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(gu=None), -1), (dict(q=None), -1), (dict(s=None), -1), (dict(dtype=3), -1), (dict(q_dtype=0), -1), (dict(rows=0), -1),
+    (dict(inter=100), -1), (dict(inter=0), -1), (dict(inter=16512), -1), (dict(limit=0.0), -1),
+    (dict(limit=float("nan")), -1), (dict(q_dtype=3, pow2=1), -1), (dict(gu=A + 8), -2), (dict(gu=A + 1, q_dtype=3), -2),
+    (dict(row_weight=A * 16 + 2), -2), (dict(q=A + 4000), -1)])
+def test_swiglu_quant_refuses(change, code):
+    assert _code("dsmoe_swiglu_quant", *{**SWIGLU, **change}.values()) == code
+
+
+GEMM = dict(a=A, a_s=2 * A, M=4, K=64, b=3 * A, b_s=4 * A, N=32, out=5 * A, out_dtype=1, stream=None)
+GROUPED = dict(a=A, a_s=2 * A, M=4, K=64, b=3 * A, b_s=4 * A, n_experts=3, N=32, offsets=6 * A, out=5 * A, out_dtype=1, stream=None)
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(a=None), -1), (dict(a_s=None), -1), (dict(b=None), -1), (dict(b_s=None), -1), (dict(out=None), -1), (dict(M=0), -1),
+    (dict(N=0), -1), (dict(K=0), -1), (dict(K=24), -1), (dict(K=131072), -1), (dict(M=1 << 31), -1), (dict(N=1 << 31), -1),
+    (dict(out_dtype=2), -1), (dict(a=A + 8), -2), (dict(b=A + 8), -2), (dict(a_s=2 * A + 1), -2), (dict(out=5 * A + 1), -2)])
+def test_int8_gemm_refuses(change, code):
+    assert _code("dsmoe_int8_gemm", *{**GEMM, **change}.values()) == code
+    assert _code("dsmoe_int8_grouped_gemm", *{**GROUPED, **change}.values()) == code
+
+
+@pytest.mark.parametrize("change,code", [(dict(offsets=None), -1), (dict(n_experts=0), -1), (dict(n_experts=1025), -1),
+                                         (dict(offsets=6 * A + 2), -2), (dict(n_experts=1024, N=1 << 21), -1)])
+def test_int8_grouped_gemm_refuses(change, code):
+    assert _code("dsmoe_int8_grouped_gemm", *{**GROUPED, **change}.values()) == code
+
+
+def test_token_entry_points_refuse():
+    sort = dict(idx=A, P=4, k=2, n_experts=8, pos=2 * A, src=3 * A, offsets=4 * A, stream=None)
+    for change, code in [(dict(idx=None), -1), (dict(pos=None), -1), (dict(src=None), -1), (dict(offsets=None), -1),
+                         (dict(P=0), -1), (dict(k=0), -1), (dict(k=65), -1), (dict(n_experts=0), -1), (dict(n_experts=1025), -1),
+                         (dict(P=1 << 30), -1), (dict(P=1 << 40, k=64), -1), (dict(idx=A + 4), -2), (dict(pos=A + 2), -2)]:
+        assert _code("dsmoe_sort_tokens", *{**sort, **change}.values()) == code, change
+    disp = dict(x=A, s=None, pos=2 * A, offsets=3 * A, n_experts=8, P=4, k=2, row_bytes=64, xs=4 * A, ss=None, stream=None)
+    for change, code in [(dict(x=None), -1), (dict(xs=None), -1), (dict(pos=None), -1), (dict(offsets=None), -1),
+                         (dict(s=A), -1), (dict(ss=A), -1), (dict(row_bytes=0), -1), (dict(row_bytes=1 << 31), -1),
+                         (dict(pos=2 * A + 1), -2)]:
+        assert _code("dsmoe_dispatch_rows", *{**disp, **change}.values()) == code, change
+    comb = dict(ys=A, dtype=1, pos=2 * A, wt=None, P=4, k=2, width=64, y=3 * A, stream=None)
+    for change, code in [(dict(ys=None), -1), (dict(y=None), -1), (dict(pos=None), -1), (dict(dtype=2), -1), (dict(width=0), -1),
+                         (dict(width=1 << 29), -1), (dict(ys=A + 1), -2), (dict(wt=A + 1), -2)]:
+        assert _code("dsmoe_combine_rows", *{**comb, **change}.values()) == code, change
+    grad = dict(dy=A, ys=2 * A, dtype=1, pos=3 * A, wt=4 * A, offsets=5 * A, n_experts=8, P=4, k=2, width=64, dys=6 * A,
+                dwt=7 * A, stream=None)
+    for change, code in [(dict(dy=None), -1), (dict(ys=None), -1), (dict(pos=None), -1), (dict(offsets=None), -1),
+                         (dict(dys=None, dwt=None), -1), (dict(dtype=3), -1), (dict(width=0), -1), (dict(dys=A + 1), -2),
+                         (dict(dwt=A + 2), -2)]:
+        assert _code("dsmoe_combine_grad", *{**grad, **change}.values()) == code, change
+
+
+def test_python_surface_takes_cuda_tensors_only():
+    import dsmoe
+    x, w = torch.zeros(2, 128), torch.ones(128)
+    q, s = torch.zeros(2, 128, dtype=torch.int8), torch.ones(2)
+    order = dsmoe.TokenOrder(torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32),
+                             torch.zeros(3, dtype=torch.int32))
+    for call in (lambda: dsmoe.rms_norm_quant(x, w), lambda: dsmoe.swiglu_quant(x), lambda: dsmoe.int8_gemm(q, s, q, s),
+                 lambda: dsmoe.int8_grouped_gemm(q, s, q[None], s[None], order.offsets),
+                 lambda: dsmoe.sort_tokens(torch.zeros(2, 1, dtype=torch.int64), 2),
+                 lambda: dsmoe.dispatch_tokens(x, order), lambda: dsmoe.combine_tokens(x, order)):
+        with pytest.raises(ValueError, match="CUDA"):
+            call()
+
+
+def test_kernel_surface_offers_the_operators():
+    import dsmoe
+    import kernel
+    assert kernel.int8_gemm is dsmoe.int8_gemm and kernel.rms_norm_quant is dsmoe.rms_norm_quant
+    assert kernel.swiglu_quant is dsmoe.swiglu_quant
+
+
+def test_quant_int8_channel():
+    from dsmoe.synth import quant_int8_channel
+    w = torch.randn((7, 33), generator=torch.Generator().manual_seed(0))
+    w[3] = 0.0
+    q, s = quant_int8_channel(w)
+    assert q.dtype == torch.int8 and s.shape == (7,) and int(q.abs().max()) == 127 and not q[3].any()
+    assert bool(((q.double() * s.double()[:, None] - w.double()).abs() <= s.double()[:, None] * (0.5 + 127 * 2.0 ** -22)).all())
