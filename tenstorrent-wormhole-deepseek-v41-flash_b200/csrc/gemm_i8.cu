@@ -399,6 +399,25 @@ int encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
   return DSMOE_OK;
 }
 
+// The current device's SM count and shared memory limit, and the kernels' attribute set once per device.
+int device_limits(const char* name, int* sms, int* optin) {
+  static std::atomic<int> known[64][2];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return cuda_status(name);
+  const int slot = dev & 63;
+  *sms = known[slot][0].load(std::memory_order_acquire);
+  *optin = known[slot][1].load(std::memory_order_acquire);
+  if (*sms && dev < 64) return DSMOE_OK;
+  if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess)
+    return cuda_status(name);
+  known[slot][1].store(*optin, std::memory_order_release);
+  known[slot][0].store(*sms, std::memory_order_release);
+  return DSMOE_OK;
+}
+
 int encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* m, const void* p, long long K, long long rows, int box_rows) {
   const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)K};
@@ -423,12 +442,11 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   DSMOE_REQUIRE((((uintptr_t)a_s | (uintptr_t)b_s | (uintptr_t)offsets) & 3) == 0 &&
                     ((uintptr_t)out & (out_dtype == DSMOE_DTYPE_F32 ? 3 : 1)) == 0,
                 DSMOE_ERR_ALIGN, "%s: misaligned pointer", name);
-  int dev = 0, sms = 0, optin = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess)
-    return cuda_status(name);
+  int sms = 0, optin = 0;
+  int rc = device_limits(name, &sms, &optin);
+  if (rc) return rc;
   PFN_cuTensorMapEncodeTiled_v12000 fn;
-  int rc = encoder(&fn);
+  rc = encoder(&fn);
   if (rc) return rc;
   Args a{};
   a.a_s = a_s; a.b_s = b_s; a.offsets = offsets; a.out = out;
@@ -454,7 +472,6 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   a.RS = (int)std::min<size_t>(MAXRS, (optin - fixed) / SB);
   const size_t smem = fixed + (size_t)a.RS * SB;
   auto kern = a.S > 1 ? gemm_i8_kernel<true> : gemm_i8_kernel<false>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, optin) != cudaSuccess) return cuda_status(name);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<long long>(tiles, std::max(1, sms / a.S)) * a.S));
   cfg.blockDim = dim3(NT);
