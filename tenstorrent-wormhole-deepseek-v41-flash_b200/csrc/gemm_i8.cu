@@ -31,7 +31,7 @@ namespace gemm_i8 {
 constexpr int NT = 320;       // 10 warps
 constexpr int CT = 256;       // epilogue threads
 constexpr int TM = 128;       // weight rows per tile (MMA M)
-constexpr int MAXTT = 256;    // tokens per tile (MMA N)
+constexpr int MAXTT = 256;    // accumulator columns of one tile
 constexpr int SPLIT_TT = 64;  // the same where K is split over a cluster
 constexpr int MAXRS = 12;     // ring stages
 constexpr int kMaxExperts = 1024;
@@ -81,6 +81,18 @@ __device__ __forceinline__ void ld16(uint32_t taddr, int (&r)[16]) {
                : "r"(taddr)
                : "memory");
 }
+__device__ __forceinline__ void ld32(uint32_t taddr, int (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+               "tcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+                 "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+                 "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr)
+               : "memory");
+}
 // The same address in the shared memory of another CTA of the cluster.
 __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -96,20 +108,148 @@ __device__ __forceinline__ int peer_ld(uint32_t addr) {
   return v;
 }
 // mbar_wait whose success also orders the other CTAs' writes before their arrivals.
+__device__ __forceinline__ bool cluster_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+  if (cluster_test(bar, parity)) return true;
   const uint64_t t0 = globaltimer_ns();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok) return true;
+  while (!cluster_test(bar, parity)) {
     if (globaltimer_ns() - t0 > limit_ns) return false;
   }
+  return true;
 }
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Groups of ceil(rows / TT) token tiles each, prefix over experts (every thread of the CTA calls this; the
+// caller synchronizes before the tables are read). Offsets that do not rise from 0 to at most M describe no
+// groups: no tile runs and the whole output is filled with NaN.
+struct Groups {
+  int tiles;   // of all groups
+  int behind;  // first row of no group
+  float fill;  // what the rows from there on hold
+};
+__device__ __forceinline__ Groups setup_groups(const Args& a, int* first, int* pre, int* wsum) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (!a.offsets) {
+    const int mt = (a.M + a.TT - 1) / a.TT;
+    if (tid == 0) {
+      first[0] = pre[0] = 0;
+      first[1] = a.M;
+      pre[1] = mt;
+    }
+    return Groups{mt * a.NTN, a.M, 0.f};
+  }
+  int bad = 0;
+  for (int e = tid; e <= a.E; e += NT) {
+    const int o = a.offsets[e];
+    first[e] = o;
+    bad |= o < (e ? a.offsets[e - 1] : 0) || o > (e ? a.M : 0);
+  }
+  bad = __syncthreads_or(bad);
+  int carry = 0;
+  for (int e0 = 0; e0 < a.E; e0 += NT) {
+    const int e = e0 + tid;
+    int inc = e < a.E && !bad ? (first[e + 1] - first[e] + a.TT - 1) / a.TT : 0;
+    const int own = inc;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int below = carry, sum = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+      if (w < warp) below += wsum[w];
+      sum += wsum[w];
+    }
+    if (e < a.E) pre[e] = below + inc - own;
+    carry += sum;
+    __syncthreads();
+  }
+  if (tid == 0) pre[a.E] = carry;
+  return Groups{carry * a.NTN, bad ? 0 : first[a.E], bad ? __int_as_float(0x7FC00000) : 0.f};
+}
+
+// Tile -> expert, channels, tokens. Tiles of one expert are neighbours, the tokens of one weight tile in a
+// row, so its bytes are in L2 when they are read again; a group's rows are spread evenly over its tiles, in
+// steps of STEP.
+template <int STEP>
+__device__ __forceinline__ Tile locate_tile(const Args& a, const int* first, const int* pre, int tile, int rows_w) {
+  int lo = 0, hi = a.E;  // the expert with pre[e] NTN <= tile < pre[e + 1] NTN
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (pre[mid] * a.NTN <= tile) lo = mid;
+    else hi = mid;
+  }
+  const int mt = pre[lo + 1] - pre[lo], at = tile - pre[lo] * a.NTN;
+  const int rows = first[lo + 1] - first[lo];
+  const int per = ((rows + mt - 1) / mt + STEP - 1) / STEP * STEP;
+  const int m = (at % mt) * per;
+  return Tile{lo, at / mt * rows_w, first[lo] + m, max(min(per, rows - m), 0)};
+}
+
+__device__ __forceinline__ void store_out(const Args& a, long long t, int n, float v) {
+  const long long o = t * a.N + n;
+  if (a.out_f32) reinterpret_cast<float*>(a.out)[o] = v;
+  else reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
+}
+
+// Accumulators of this warp's 32 channels and every other 32 tokens from 32 `half` on -> out. sc: the tokens'
+// scales in shared memory (padded to 32). The store of one token is 32 neighbouring channels.
+template <typename T>
+__device__ __forceinline__ void drain(const Args& a, uint32_t tq, int half, int cols, long long m0, int n, float bs,
+                                      const float* sc, bool ok) {
+  if (!ok) bs = __int_as_float(0x7FC00000);
+  const bool live = n < a.N;
+  T* p = reinterpret_cast<T*>(a.out) + (m0 + 32 * half) * a.N + n;
+  for (int c0 = 32 * half; c0 < cols; c0 += 64, p += 64LL * a.N) {
+    int v[32];
+    ld32(tq + (uint32_t)c0, v);
+    T* o = p;
+    if (live && c0 + 32 <= cols) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(sc + c0 + i);
+        o[0] = (T)((float)v[i] * bs * s.x);
+        o += a.N;
+        o[0] = (T)((float)v[i + 1] * bs * s.y);
+        o += a.N;
+        o[0] = (T)((float)v[i + 2] * bs * s.z);
+        o += a.N;
+        o[0] = (T)((float)v[i + 3] * bs * s.w);
+        o += a.N;
+      }
+    } else if (live) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (c0 + i < cols) o[0] = (T)((float)v[i] * bs * sc[c0 + i]);
+        o += a.N;
+      }
+    }
+  }
+}
+__device__ __forceinline__ void drain(const Args& a, uint32_t tq, int half, int cols, long long m0, int n, float bs,
+                                      const float* sc, bool ok) {
+  if (a.out_f32) drain<float>(a, tq, half, cols, m0, n, bs, sc, ok);
+  else drain<__nv_bfloat16>(a, tq, half, cols, m0, n, bs, sc, ok);
+}
+
+// Rows behind the last group, by the epilogue threads of the whole grid.
+__device__ __forceinline__ void fill_behind(const Args& a, const Groups& g, int ct) {
+  const long long to = (long long)a.M * a.N;
+  for (long long i = (long long)g.behind * a.N + (long long)blockIdx.x * CT + ct; i < to; i += (long long)gridDim.x * CT) {
+    if (a.out_f32) reinterpret_cast<float*>(a.out)[i] = g.fill;
+    else reinterpret_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(g.fill);
+  }
 }
 
 template <bool SPLIT>
@@ -126,7 +266,8 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
   uint64_t* pfull = acce + 2;        // [2] SPLIT: every CTA's partial written
   uint64_t* pempty = pfull + 2;      // [2] SPLIT: this CTA's partial read by every CTA
   uint64_t* mdone = pempty + 2;      // [1] no MMA in flight
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(mdone + 1);
+  float* scales = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(mdone + 1) + 15) & ~(uintptr_t)15);  // [2][SPLIT_TT]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(scales + 2 * SPLIT_TT);
   volatile int* abortf = reinterpret_cast<volatile int*>(tslot + 1);
   int* wsum = reinterpret_cast<int*>(tslot + 2);  // [10]
   int* first = wsum + 10;            // [E + 1] first row of each group
@@ -157,52 +298,8 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // groups of ceil(rows / TT) tiles, prefix over experts. Offsets that do not rise from 0 to at most M
-  // describe no groups: no tile runs and the whole output is NaN.
-  int tiles, behind = a.M;
-  float fill = 0.f;
-  if (a.offsets) {
-    int bad = 0;
-    for (int e = tid; e <= a.E; e += NT) {
-      const int o = a.offsets[e];
-      first[e] = o;
-      bad |= o < (e ? a.offsets[e - 1] : 0) || o > (e ? a.M : 0);
-    }
-    bad = __syncthreads_or(bad);
-    int carry = 0;
-    for (int e0 = 0; e0 < a.E; e0 += NT) {
-      const int e = e0 + tid;
-      int inc = e < a.E && !bad ? (first[e + 1] - first[e] + a.TT - 1) / a.TT : 0;
-      const int own = inc;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) wsum[warp] = inc;
-      __syncthreads();
-      int below = carry, sum = 0;
-      for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) below += wsum[w];
-        sum += wsum[w];
-      }
-      if (e < a.E) pre[e] = below + inc - own;
-      carry += sum;
-      __syncthreads();
-    }
-    if (tid == 0) pre[a.E] = carry;
-    tiles = carry * a.NTN;
-    behind = bad ? 0 : first[a.E];
-    if (bad) fill = __int_as_float(0x7FC00000);
-  } else {
-    if (tid == 0) {
-      first[0] = 0;
-      first[1] = a.M;
-      pre[0] = 0;
-      pre[1] = (a.M + a.TT - 1) / a.TT;
-    }
-    tiles = (a.M + a.TT - 1) / a.TT * a.NTN;
-  }
+  const Groups g = setup_groups(a, first, pre, wsum);
+  const int tiles = g.tiles;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (SPLIT) cluster_sync();  // every CTA's barriers exist before the first remote arrival
@@ -216,21 +313,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
     }
     return true;
   };
-  // tile -> expert, channels, tokens. Tiles of one expert are neighbours, the tokens of one weight tile
-  // in a row, so its bytes are in L2 when they are read again.
-  auto locate = [&](int tile) -> Tile {
-    int lo = 0, hi = a.E;  // the expert with pre[e] NTN <= tile < pre[e + 1] NTN
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (pre[mid] * a.NTN <= tile) lo = mid;
-      else hi = mid;
-    }
-    const int mt = pre[lo + 1] - pre[lo], at = tile - pre[lo] * a.NTN;
-    const int rows = first[lo + 1] - first[lo];
-    const int per = ((rows + mt - 1) / mt + 15) & ~15;  // the group's rows spread evenly over its tiles
-    const int m = (at % mt) * per;
-    return Tile{lo, at / mt * TM, first[lo] + m, max(min(per, rows - m), 0)};
-  };
+  auto locate = [&](int tile) -> Tile { return locate_tile<16>(a, first, pre, tile, TM); };
 
   if (warp == 0) {
     if (lane == 0) {
@@ -292,34 +375,27 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
     const int qd = warp & 3, half = (warp - 2) >> 2;
     const int row_l = 32 * qd + lane;
     const float nanv = __int_as_float(0x7FC00000);
-    auto store = [&](long long t, int n, float v) {
-      const long long o = t * a.N + n;
-      if (a.out_f32) reinterpret_cast<float*>(a.out)[o] = v;
-      else reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
-    };
+    auto store = [&](long long t, int n, float v) { store_out(a, t, n, v); };
     int tc = 0;
     bool ok = true;
     for (int tile = cid; tile < tiles; tile += ncl, ++tc) {
       const Tile t = locate(tile);
       const int ac = tc & 1;
+      const int n = t.n0 + row_l;
+      float bs = 0.f;
+      float* sc = scales + ac * SPLIT_TT;
+      if (!SPLIT) {
+        // the tile's scales, while its products are still running (the other half of the buffer is being read)
+        if (n < a.N) bs = a.b_s[(long long)t.e * a.N + n];
+        if (ct < SPLIT_TT) sc[ct] = ct < t.cols ? a.a_s[t.m0 + ct] : 0.f;
+        named_bar_sync(1, CT);
+      }
       ok = ok && wait(&accf[ac], (tc >> 1) & 1);
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       const int groups = (t.cols + 15) >> 4;  // 16 tokens at a time, the two warps of a quadrant in turn
       const uint32_t tq = tmem + ((uint32_t)(32 * qd) << 16) + (uint32_t)(ac * MAXTT);
       if (!SPLIT) {
-        const int n = t.n0 + row_l;
-        const float bs = n < a.N ? a.b_s[(long long)t.e * a.N + n] : 0.f;
-        for (int g = half; g < groups; g += 2) {
-          int v[16];
-          ld16(tq + 16u * g, v);
-          const int c = 16 * g + (lane & 15);
-          const float as = c < t.cols ? a.a_s[t.m0 + c] : 0.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float sc = __shfl_sync(0xffffffffu, as, i);
-            if (n < a.N && 16 * g + i < t.cols) store(t.m0 + 16 * g + i, n, ok ? (float)v[i] * sc * bs : nanv);
-          }
-        }
+        drain(a, tq, half, t.cols, t.m0, n, bs, sc, ok);
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&acce[ac]);
@@ -329,11 +405,11 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
           ok = cluster_wait(&pempty[ac], ((tc >> 1) - 1) & 1, kWaitNs);
           if (!ok) *abortf = 1;
         }
-        for (int g = half; g < groups; g += 2) {
+        for (int c16 = half; c16 < groups; c16 += 2) {
           int v[16];
-          ld16(tq + 16u * g, v);
+          ld16(tq + 16u * c16, v);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mine[(16 * g + i) * TM + row_l] = v[i];
+          for (int i = 0; i < 16; ++i) mine[(16 * c16 + i) * TM + row_l] = v[i];
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -346,29 +422,22 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
           if (!ok) *abortf = 1;
         }
         // this CTA finishes channels rank TM / S .. of the tile, for every token
-        const int rows = TM / S, r = rank * rows + ct % rows, n = t.n0 + r;
-        if (n < a.N) {
-          const float bs = a.b_s[(long long)t.e * a.N + n];
+        const int rows = TM / S, r = rank * rows + ct % rows, nr = t.n0 + r;
+        if (nr < a.N) {
+          bs = a.b_s[(long long)t.e * a.N + nr];
           for (int c = ct / rows; c < t.cols; c += CT / rows) {
             const uint32_t at = smem_u32(mine + c * TM + r);
             int sum = 0;
             if (ok)
               for (int z = 0; z < S; ++z) sum += peer_ld(peer_addr(at, (uint32_t)z));
-            store(t.m0 + c, n, ok ? (float)sum * a.a_s[t.m0 + c] * bs : nanv);
+            store(t.m0 + c, nr, ok ? (float)sum * a.a_s[t.m0 + c] * bs : nanv);
           }
         }
         named_bar_sync(1, CT);
         if (ct < S) peer_arrive(&pempty[ac], (uint32_t)ct);
       }
     }
-    // rows behind the last group
-    {
-      const long long from = (long long)behind * a.N, to = (long long)a.M * a.N;
-      for (long long i = from + (long long)blockIdx.x * CT + ct; i < to; i += (long long)gridDim.x * CT) {
-        if (a.out_f32) reinterpret_cast<float*>(a.out)[i] = fill;
-        else reinterpret_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16_rn(fill);
-      }
-    }
+    fill_behind(a, g, ct);
   }
   __syncwarp();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -377,6 +446,197 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ CTA pairs
+// Many tokens: two CTAs of a cluster work as a pair (cta_group::2) on a tile of 256 weight rows x up to 512
+// tokens. Each CTA loads its own 128 weight rows and half of the token rows, the leader's MMA (M 256, N up to
+// 256, one for each half of the tile's tokens) reads both CTAs' shared memory and writes each CTA's 128 rows
+// of accumulators into that CTA's tensor memory.
+constexpr int PTT = 512;                   // tokens per tile
+constexpr int PSB = TM * 128 + PTT / 2 * 128;  // stage bytes of one CTA: 16 KB of weights, 32 KB of tokens
+constexpr int PRS = 4;                     // stages
+constexpr int PBR = 64;                    // token rows of one load
+
+__device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Arrives at the barrier of both CTAs when the pair's MMAs so far are complete.
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+               ::"r"(smem_u32(bar)), "h"((unsigned short)3) : "memory");
+}
+// A load into this CTA's shared memory that reports to a barrier of the pair's leader.
+__device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* tm, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) uint8_t gsm[];
+  uint8_t* ring = gsm + ((1024 - (smem_u32(gsm) & 1023)) & 1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + PRS * PSB);
+  uint64_t* full = bars;           // [PRS] leader: both CTAs' stage landed
+  uint64_t* empty = full + PRS;    // [PRS] stage read by its MMAs
+  uint64_t* accf = empty + PRS;    // [2] half of the tensor memory: accumulators complete
+  uint64_t* acce = accf + 2;       // [2] leader: accumulators read by both CTAs (8 warps each)
+  uint64_t* mdone = acce + 2;      // [1] no MMA in flight
+  float* scales = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(mdone + 1) + 15) & ~(uintptr_t)15);  // [2][256]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(scales + 2 * 256);
+  volatile int* abortf = reinterpret_cast<volatile int*>(tslot + 1);
+  int* wsum = reinterpret_cast<int*>(tslot + 2);  // [10]
+  int* first = wsum + 10;          // [E + 1] first row of each group
+  int* pre = first + a.E + 1;      // [E + 1] tiles before each group
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = blockIdx.x & 1, cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
+  if (tid == 0) {
+    for (int s = 0; s < PRS; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&accf[s], 1);
+      mbar_init(&acce[s], 16);
+    }
+    mbar_init(mdone, 1);
+    *abortf = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  const Groups g = setup_groups(a, first, pre, wsum);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers and tensor memory exist
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = *tslot;
+  auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
+    if (*abortf) return false;
+    if (!cluster_wait(bar, par, kWaitNs)) {
+      *abortf = 1;
+      return false;
+    }
+    return true;
+  };
+  auto locate = [&](int tile) -> Tile { return locate_tile<32>(a, first, pre, tile, 2 * TM); };
+  // A tile's tokens in one or two halves of up to 256, each a multiple of 32 as the MMA wants; half h uses the
+  // next half of the tensor memory, so a tile of up to 256 tokens is stored while the next one is computed.
+  auto width = [](int cols, int h) -> int {
+    const int all = max((cols + 31) & ~31, 32);
+    return h == 0 ? min(all, 256) : max(all - 256, 0);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
+      int it = 0;
+      bool ok = true;
+      for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
+        const Tile t = locate(tile);
+        const int w0 = width(t.cols, 0), w1 = width(t.cols, 1);
+        const int nb0 = (w0 / 2 + PBR - 1) / PBR, nb1 = (w1 / 2 + PBR - 1) / PBR;
+        const int y0 = t.m0 + rank * (w0 / 2), y1 = t.m0 + w0 + rank * (w1 / 2);
+        for (int kb = 0; kb < a.nkb; ++kb, ++it) {
+          const int s = it % PRS;
+          if (it >= PRS && !wait(&empty[s], ((it / PRS) - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = ring + s * PSB;
+          if (rank == 0) mbar_expect_tx(&full[s], (uint32_t)(2 * (TM * 128 + (nb0 + nb1) * PBR * 128)));
+          const uint32_t bar = peer_addr(smem_u32(&full[s]), 0);
+          tma_2d_pair(st, &a.tb, kb * 128, t.e * a.N + t.n0 + rank * TM, bar);
+          for (int b = 0; b < nb0; ++b) tma_2d_pair(st + TM * 128 + b * PBR * 128, &a.ta, kb * 128, y0 + b * PBR, bar);
+          for (int b = 0; b < nb1; ++b) tma_2d_pair(st + TM * 128 + 16384 + b * PBR * 128, &a.ta, kb * 128, y1 + b * PBR, bar);
+        }
+      }
+      // every copy issued has landed (its MMAs have read it) before the CTA may exit
+      for (int i = it - 1; i >= 0 && i >= it - PRS; --i) cluster_wait(&empty[i % PRS], (i / PRS) & 1, kWaitNs);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc0 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(2 * TM >> 4) << 24);
+      const uint64_t da0 = desc_sw128(smem_u32(ring)), db0 = desc_sw128(smem_u32(ring + TM * 128));
+      int it = 0, slot = 0;  // slots: halves of the tensor memory used so far
+      bool ok = true;
+      for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
+        const Tile t = locate(tile);
+        const int w0 = width(t.cols, 0), w1 = width(t.cols, 1), n = w1 ? 2 : 1;
+        for (int h = 0; h < n && ok; ++h)
+          if (slot + h >= 2) ok = wait(&acce[(slot + h) & 1], (((slot + h) >> 1) - 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t id0 = idesc0 | ((uint32_t)(w0 >> 3) << 17), id1 = idesc0 | ((uint32_t)(w1 >> 3) << 17);
+        const uint32_t d0 = tmem + (uint32_t)((slot & 1) * 256), d1 = tmem + (uint32_t)(((slot + 1) & 1) * 256);
+        for (int kb = 0; kb < a.nkb; ++kb, ++it) {
+          const int s = it % PRS;
+          if (!wait(&full[s], (it / PRS) & 1)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint64_t o = (uint64_t)(s * (PSB >> 4));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mma_i8_pair(d0, da0 + o + 2u * q, db0 + o + 2u * q, id0, (kb > 0 || q > 0) ? 1u : 0u);
+          if (w1) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              mma_i8_pair(d1, da0 + o + 2u * q, db0 + o + 1024u + 2u * q, id1, (kb > 0 || q > 0) ? 1u : 0u);
+          }
+          commit_pair(&empty[s]);
+        }
+        for (int h = 0; h < n; ++h) commit_pair(&accf[(slot + h) & 1]);
+        slot += n;
+      }
+      commit_pair(mdone);  // no MMA may still run when the tensor memory is freed
+    }
+    if (lane == 0) cluster_wait(mdone, 0, 4 * kWaitNs);
+  } else {
+    const int ct = tid - 64;
+    const int qd = warp & 3, half = (warp - 2) >> 2;
+    const int row_l = 32 * qd + lane;
+    int slot = 0;
+    bool ok = true;
+    for (int tile = cid; tile < g.tiles; tile += ncl) {
+      const Tile t = locate(tile);
+      const int n = t.n0 + rank * TM + row_l;
+      const float bs = n < a.N ? a.b_s[(long long)t.e * a.N + n] : 0.f;
+      for (int h = 0; h < 2 && width(t.cols, h); ++h, ++slot) {
+        const int cols = h ? t.cols - 256 : min(t.cols, 256);
+        const long long m0 = t.m0 + 256 * h;
+        // the tokens' scales, while the products are still running (the other half of the buffer is being read)
+        float* sc = scales + (slot & 1) * 256;
+        sc[ct] = ct < cols ? a.a_s[m0 + ct] : 0.f;
+        named_bar_sync(1, CT);
+        ok = ok && wait(&accf[slot & 1], (slot >> 1) & 1);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t tq = tmem + ((uint32_t)(32 * qd) << 16) + (uint32_t)((slot & 1) * 256);
+        drain(a, tq, half, cols, m0, n, bs, sc, ok);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) peer_arrive(&acce[slot & 1], 0);
+      }
+    }
+    fill_behind(a, g, ct);
+  }
+  __syncwarp();
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other's MMAs or arrivals may reach it
+  if (warp == 1) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
 }
 
@@ -411,6 +671,7 @@ int device_limits(const char* name, int* sms, int* optin) {
   if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
       cudaDeviceGetAttribute(optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_i8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_i8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess)
     return cuda_status(name);
   known[slot][1].store(*optin, std::memory_order_release);
@@ -454,24 +715,50 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   a.nkb = (int)((K + 127) / 128);
   a.NTN = (int)((N + TM - 1) / TM);
   a.out_f32 = out_dtype == DSMOE_DTYPE_F32;
-  // tokens of a tile: the mean group's, in the next of 16, 32, 64 or 256
+  // tokens of a tile: the mean group's, in the next of 16, 32 or 64; beyond that CTA pairs
   const long long mean = offsets ? (M + E - 1) / E : M;
-  a.TT = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : MAXTT;
   const long long groups = offsets ? std::min<long long>(E, M) : 1;
+  const bool pair = mean > SPLIT_TT;
+  a.TT = mean <= 16 ? 16 : mean <= 32 ? 32 : SPLIT_TT;
+  a.S = 1;
+  a.BR = a.TT;
+  if (pair) {
+    a.NTN = (int)((N + 2 * TM - 1) / (2 * TM));
+    a.TT = PTT;
+    a.S = 2;
+    a.BR = PBR;
+    if (!offsets) {
+      // the tile width that costs least: rounds of the pairs times a tile's columns, with the time that a
+      // tile costs beside its MMAs (filling the ring, storing the last accumulators) as 64 columns
+      long long best = 0;
+      for (long long mt = (M + PTT - 1) / PTT; mt <= (M + 63) / 64; ++mt) {
+        const long long per = ((M + mt - 1) / mt + 31) / 32 * 32;
+        const long long cost = (mt * a.NTN + sms / 2 - 1) / (sms / 2) * (per + 64);
+        if (!best || cost < best) {
+          best = cost;
+          a.TT = (int)per;
+        }
+      }
+    }
+  }
   const long long tiles = a.NTN * (M / a.TT + groups);  // at most
   DSMOE_REQUIRE(tiles < (1LL << 31), DSMOE_ERR_ARG, "%s: too many tiles", name);
-  a.S = 1;
-  if (a.TT <= SPLIT_TT)
+  if (!pair)
     while (a.S < 8 && a.S * 2 <= a.nkb && tiles * a.S * 2 <= sms) a.S *= 2;
-  a.BR = std::min(a.TT, 64);
   rc = encode(fn, &a.tb, b, K, (long long)E * N, TM);
   if (!rc) rc = encode(fn, &a.ta, x, K, M, a.BR);
   if (rc) return rc;
-  const int SB = (TM + a.TT) * 128;
-  const size_t fixed = 1024 + (a.S > 1 ? 2 * a.TT * TM * 4 : 0) + (2 * MAXRS + 9) * 8 + 48 + 2 * (E + 1) * 4 + 64;
-  a.RS = (int)std::min<size_t>(MAXRS, (optin - fixed) / SB);
-  const size_t smem = fixed + (size_t)a.RS * SB;
-  auto kern = a.S > 1 ? gemm_i8_kernel<true> : gemm_i8_kernel<false>;
+  const size_t tables = (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
+  size_t smem;
+  if (pair) {
+    smem = 1024 + PRS * PSB + tables;
+  } else {
+    const int SB = (TM + a.TT) * 128;
+    const size_t fixed = 1024 + (a.S > 1 ? 2 * a.TT * TM * 4 : 0) + tables;
+    a.RS = (int)std::min<size_t>(MAXRS, (optin - fixed) / SB);
+    smem = fixed + (size_t)a.RS * SB;
+  }
+  auto kern = pair ? gemm_i8_pair_kernel : a.S > 1 ? gemm_i8_kernel<true> : gemm_i8_kernel<false>;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(std::min<long long>(tiles, std::max(1, sms / a.S)) * a.S));
   cfg.blockDim = dim3(NT);
