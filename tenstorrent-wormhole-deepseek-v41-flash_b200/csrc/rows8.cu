@@ -18,6 +18,8 @@ namespace rows8 {
 
 constexpr float kAmaxFloor = 1e-4f;
 constexpr int kMaxHidden = 16384;
+constexpr int kStages = 3;              // rows in a persistent CTA's ring
+constexpr int kMaxSmem = 227 * 1024;
 
 struct Args {
   const void* x;      // norm: [rows][n]; swiglu: [rows][2n] (g | u)
@@ -34,25 +36,35 @@ struct Args {
   float eps, limit;
 };
 
+// A chunk as loaded, and its values: bf16 stays packed in registers until it is used.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_chunk(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = (float)p[0];
-  } else if constexpr (sizeof(T) == 2) {
-    static_assert(VEC == 8, "");
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+struct Raw {
+  T v;  // VEC == 1
+  __device__ __forceinline__ void load(const T* p) { v = p[0]; }
+  __device__ __forceinline__ void zero() { v = (T)0.f; }
+  __device__ __forceinline__ void get(float (&o)[VEC]) const { o[0] = (float)v; }
+};
+template <>
+struct Raw<__nv_bfloat16, 8> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
-  } else {
-    static_assert(VEC == 4, "");
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
   }
-}
+};
+template <>
+struct Raw<float, 4> {
+  float4 u;
+  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void zero() { u = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = u.x; o[1] = u.y; o[2] = u.z; o[3] = u.w; }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void store_chunk(T* p, const float (&v)[VEC]) {
@@ -100,11 +112,20 @@ __device__ __forceinline__ void load_w(const void* w, int w_bf16, int at, float 
   }
 }
 
-// |v| as an integer that orders like the value, with infinities and NaN above every finite one
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+// Minimum and maximum that keep a NaN.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-__device__ __forceinline__ float scale_of(float amax, float top, int pow2) {
-  float s = (amax < kAmaxFloor ? kAmaxFloor : amax) / top;  // a NaN stays
+__device__ __forceinline__ float scale_of(float amax, float inv_top, int pow2) {
+  float s = (amax < kAmaxFloor ? kAmaxFloor : amax) * inv_top;  // a NaN stays
   if (pow2) {
     int e;
     const float m = frexpf(s, &e);
@@ -122,21 +143,27 @@ __device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
   return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
 }
 
-// One block reduction per row: sum and integer maximum over the row's tpr threads.
+// One block reduction per row: sum and maximum (not negative) over the row's tpr threads. Numbers that are not
+// negative order like their bits, with infinity and NaN on top, so the maximum is an integer one.
 template <bool SUM, bool MAX>
-__device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, int tpr) {
+__device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr, int turn) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if (MAX) top = __reduce_max_sync(0xffffffffu, top);
-  if (tpr == 32) return;
-  __shared__ float ssum[32];
-  __shared__ uint32_t smax[32];
+  if (MAX) top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7FFFFFFFu));
+  if (tpr == 32 && blockDim.x == 32) {
+    __syncwarp();
+    return;
+  }
+  __shared__ float ssums[2][32];  // a second reduction (turn 1) may begin while the first is being read
+  __shared__ uint32_t smaxs[2][32];
+  float* ssum = ssums[turn];
+  uint32_t* smax = smaxs[turn];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tpr >> 5, w0 = warp / nw * nw;
   if (lane == 0) {
     if (SUM) ssum[warp] = sum;
-    if (MAX) smax[warp] = top;
+    if (MAX) smax[warp] = __float_as_uint(top);
   }
   __syncthreads();
   if (SUM) {
@@ -144,26 +171,26 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& top, int tpr) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  if (MAX) top = __reduce_max_sync(0xffffffffu, lane < nw ? smax[w0 + lane] : 0u);
+  if (MAX) top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nw ? smax[w0 + lane] : 0u));
 }
 
-// v * mul to 8 bits with its scales; top: the row's amax of v (int8), mul: what v still lacks.
+// v * mul to 8 bits with its scales; top: the row's max |v| (int8), mul: the row's factor that v still lacks.
 template <int VEC, int NV, bool FP8>
-__device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][VEC], float mul, uint32_t top, long long row,
+__device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][VEC], float mul, float top, long long row,
                                             int t, bool live) {
   if constexpr (FP8) {
     uint8_t* q = reinterpret_cast<uint8_t*>(a.q) + row * a.n;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = j * a.tpr + t;
-      uint32_t m = 0;
+      float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) m = max(m, abs_bits(v[j][i]));
+      for (int i = 0; i < VEC; ++i) m = max_nan(m, fabsf(v[j][i]));
       // the 128 values of a block are 16 (bf16) or 32 (fp32) neighbouring lanes' chunks
 #pragma unroll
-      for (int o = 64 / VEC; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float s = scale_of(__uint_as_float(m) * mul, 448.0f, a.pow2);
-      const float f = mul * __frcp_rn(s);
+      for (int o = 64 / VEC; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float s = scale_of(m * fabsf(mul), 1.0f / 448.0f, a.pow2);
+      const float f = mul * __fdividef(1.0f, s);
       if (live && c < a.nchunk) {
         if ((c * VEC) % 128 == 0) a.s[row * (a.n / 128) + c * VEC / 128] = s;
         const uint32_t lo = f32x2_to_e4m3x2(v[j][0] * f, v[j][1] * f) | (f32x2_to_e4m3x2(v[j][2] * f, v[j][3] * f) << 16);
@@ -176,8 +203,8 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
       }
     }
   } else {
-    const float s = scale_of(__uint_as_float(top) * mul, 127.0f, 0);
-    const float f = s == s ? mul * __frcp_rn(s) : 0.f;
+    const float s = scale_of(top * fabsf(mul), 1.0f / 127.0f, 0);
+    const float f = mul * __fdividef(1.0f, s);
     if (!live) return;
     if (t == 0) a.s[row] = s;
     uint8_t* q = reinterpret_cast<uint8_t*>(a.q) + row * a.n;
@@ -199,66 +226,144 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
   }
 }
 
+// One row in registers: residual added and stored, squares and |r w| reduced; v holds r w afterwards.
+template <typename T, int VEC, int NV, bool FP8>
+__device__ __forceinline__ void norm_row(const Args& a, const Raw<T, VEC> (&x)[NV], const Raw<T, VEC> (&r)[NV],
+                                         float (&v)[NV][VEC], float& sum, float& top, long long at, int t, bool live) {
+  sum = 0.f;
+  top = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * a.tpr + t;
+    x[j].get(v[j]);
+    if (live && c < a.nchunk) {
+      if (a.res) {
+        float y[VEC];
+        r[j].get(y);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] = round_to<T>(v[j][i] + y[i]);
+        if (a.res_out) store_chunk<T, VEC>(reinterpret_cast<T*>(a.res_out) + at + c * VEC, v[j]);
+      }
+      float w[VEC];
+      load_w<VEC>(a.w, a.w_bf16, c * VEC, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        sum = fmaf(v[j][i], v[j][i], sum);
+        v[j][i] *= w[i];
+        if (!FP8) top = max_nan(top, fabsf(v[j][i]));
+      }
+    }
+  }
+}
+
+template <typename T, int VEC, int NV>
+__device__ __forceinline__ void store_normed(const Args& a, const float (&v)[NV][VEC], float rstd, long long at, int t, bool live) {
+  if (!a.normed || !live) return;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = j * a.tpr + t;
+    if (c >= a.nchunk) continue;
+    float y[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) y[i] = v[j][i] * rstd;
+    store_chunk<T, VEC>(reinterpret_cast<T*>(a.normed) + at + c * VEC, y);
+  }
+}
+
 template <typename T, int VEC, int NV, bool FP8>
 __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
   const int g = threadIdx.x / a.tpr, t = threadIdx.x % a.tpr;
   const long long row = (long long)blockIdx.x * a.rpc + g;
   const bool live = row < a.rows;
   const long long at = row * a.n;
-  float v[NV][VEC], y[NV][VEC];
-  const T* x = reinterpret_cast<const T*>(a.x) + at;
-  const T* r = reinterpret_cast<const T*>(a.res) + at;
+  Raw<T, VEC> x[NV], r[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = j * a.tpr + t;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[j][i] = y[j][i] = 0.f;
+    x[j].zero();
+    r[j].zero();
     if (live && c < a.nchunk) {
-      load_chunk<T, VEC>(x + c * VEC, v[j]);
-      if (a.res) load_chunk<T, VEC>(r + c * VEC, y[j]);
+      x[j].load(reinterpret_cast<const T*>(a.x) + at + c * VEC);
+      if (a.res) r[j].load(reinterpret_cast<const T*>(a.res) + at + c * VEC);
     }
   }
-  float sum = 0.f;
-  uint32_t top = 0;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = j * a.tpr + t;
-    if (live && c < a.nchunk) {
-      float w[VEC];
-      load_w<VEC>(a.w, a.w_bf16, c * VEC, w);
-      if (a.res) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = round_to<T>(v[j][i] + y[j][i]);
-        if (a.res_out) store_chunk<T, VEC>(reinterpret_cast<T*>(a.res_out) + at + c * VEC, v[j]);
-      }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        sum = fmaf(v[j][i], v[j][i], sum);
-        v[j][i] *= w[i];
-        if (!FP8) top = max(top, abs_bits(v[j][i]));
-      }
-    }
-  }
-  row_reduce<true, !FP8>(sum, top, a.tpr);
+  float v[NV][VEC], sum;
+  float top;
+  norm_row<T, VEC, NV, FP8>(a, x, r, v, sum, top, at, t, live);
+  row_reduce<true, !FP8>(sum, top, a.tpr, 0);
   const float rstd = 1.0f / sqrtf(sum / (float)a.n + a.eps);
-  if (a.normed && live) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = j * a.tpr + t;
-      if (c >= a.nchunk) continue;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) y[j][i] = v[j][i] * rstd;
-      store_chunk<T, VEC>(reinterpret_cast<T*>(a.normed) + at + c * VEC, y[j]);
-    }
-  }
+  store_normed<T, VEC, NV>(a, v, rstd, at, t, live);
   quant_store<VEC, NV, FP8>(a, v, rstd, top, row, t, live);
 }
 
-// silu(g) u with g <= limit, |u| <= limit; comparisons keep a NaN.
+// Many rows: a persistent CTA walks rows blockIdx.x + i gridDim.x while bulk copies bring the next ones into a
+// ring of shared memory, so loads stay in flight over the reductions and stores of the rows before.
+constexpr uint64_t kWaitNs = 1000000000ull;
+
+template <typename T, int VEC, int NV, bool FP8>
+__global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ uint64_t full[kStages];
+  const int t = threadIdx.x, terms = a.res ? 2 : 1;
+  const uint32_t row_bytes = (uint32_t)(a.n * sizeof(T));
+  if (t == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  auto fetch = [&](long long row, int s) {
+    uint8_t* st = sm + (size_t)s * terms * row_bytes;
+    mbar_expect_tx(&full[s], terms * row_bytes);
+    bulk_g2s(st, reinterpret_cast<const T*>(a.x) + row * a.n, row_bytes, &full[s]);
+    if (a.res) bulk_g2s(st + row_bytes, reinterpret_cast<const T*>(a.res) + row * a.n, row_bytes, &full[s]);
+  };
+  const long long step = gridDim.x;
+  if (t == 0)
+    for (int s = 0; s < kStages; ++s)
+      if (blockIdx.x + s * step < a.rows) fetch(blockIdx.x + s * step, s);
+  int i = 0;
+  for (long long row = blockIdx.x; row < a.rows; row += step, ++i) {
+    const int s = i % kStages;
+    const bool ok = mbar_wait(&full[s], (i / kStages) & 1, kWaitNs);
+    const T* st = reinterpret_cast<const T*>(sm + (size_t)s * terms * row_bytes);
+    Raw<T, VEC> x[NV], r[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = j * a.tpr + t;
+      x[j].zero();
+      r[j].zero();
+      if (c < a.nchunk) {
+        x[j].load(st + c * VEC);
+        if (a.res) r[j].load(st + a.n + c * VEC);
+      }
+    }
+    float v[NV][VEC], sum;
+    float top;
+    norm_row<T, VEC, NV, FP8>(a, x, r, v, sum, top, row * a.n, t, true);
+    row_reduce<true, !FP8>(sum, top, a.tpr, i & 1);  // its barrier: every thread has read the stage
+    if (t == 0 && row + kStages * step < a.rows) fetch(row + kStages * step, s);
+    // an expired wait leaves a row of NaN
+    const float rstd = ok ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : __int_as_float(0x7FC00000);
+    store_normed<T, VEC, NV>(a, v, rstd, row * a.n, t, true);
+    quant_store<VEC, NV, FP8>(a, v, rstd, top, row, t, true);
+  }
+}
+
+// silu(g) u with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + d ln 2) with t = -g log2(e) rounded and d what the
+// rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all that is
+// approximated; the argument's own rounding would cost |g| units. exp's argument stops at 87, where silu(g) is
+// below 1e-35, so that the reciprocal stays a normal number.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  g = g > limit ? limit : g;
-  u = u > limit ? limit : (u < -limit ? -limit : u);
-  return g / (1.0f + expf(-g)) * u;
+  g = min_nan(g, limit);
+  u = max_nan(min_nan(u, limit), -limit);
+  constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+  const float a = max_nan(g, -87.0f);
+  const float t = -a * kLog2e, d = fmaf(-a, kLog2e, -t);
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e = 1.0f + fmaf(e, d * kLn2, e);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
+  return g * r * u;
 }
 
 template <typename T, int VEC, int NV, bool FP8>
@@ -267,31 +372,39 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
   const long long row = (long long)blockIdx.x * a.rpc + gidx;
   const bool live = row < a.rows;
   const T* g = reinterpret_cast<const T*>(a.x) + row * 2 * a.n;
-  const T* u = g + a.n;
-  float v[NV][VEC], y[NV][VEC];
+  Raw<T, VEC> x[NV], y[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = j * a.tpr + t;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[j][i] = y[j][i] = 0.f;
+    x[j].zero();
+    y[j].zero();
     if (live && c < a.nchunk) {
-      load_chunk<T, VEC>(g + c * VEC, v[j]);
-      load_chunk<T, VEC>(u + c * VEC, y[j]);
+      x[j].load(g + c * VEC);
+      y[j].load(g + a.n + c * VEC);
     }
   }
   const float wr = live && a.w ? reinterpret_cast<const float*>(a.w)[row] : 1.0f;
-  uint32_t top = 0;
-  float none = 0.f;
+  float v[NV][VEC], top = 0.f, none = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
+    float u[VEC];
+    x[j].get(v[j]);
+    y[j].get(u);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      v[j][i] = swiglu(v[j][i], y[j][i], a.limit) * wr;
-      if (!FP8) top = max(top, abs_bits(v[j][i]));
+      v[j][i] = swiglu(v[j][i], u[i], a.limit);
+      if (!FP8) top = max_nan(top, fabsf(v[j][i]));
     }
   }
-  if (!FP8) row_reduce<false, true>(none, top, a.tpr);
-  quant_store<VEC, NV, FP8>(a, v, 1.0f, top, row, t, live);
+  if (!FP8) row_reduce<false, true>(none, top, a.tpr, 0);
+  quant_store<VEC, NV, FP8>(a, v, wr, top, row, t, live);
+}
+
+int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
 }
 
 template <bool NORM, typename T, int VEC, int NV, bool FP8>
@@ -301,23 +414,54 @@ void launch(const Args& a, cudaStream_t st) {
   else swiglu_kernel<T, VEC, NV, FP8><<<(unsigned)grid, a.tpr * a.rpc, 0, st>>>(a);
 }
 
+template <typename T, int NV, bool FP8>
+void launch_stream(const Args& a, int ctas, size_t smem, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  auto k = norm_stream_kernel<T, V, NV, FP8>;
+  if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  k<<<ctas, a.tpr, smem, st>>>(a);
+}
+
 template <bool NORM, typename T>
 int run(Args& a, bool fp8, bool wide, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const int vec = wide ? V : 1;
   a.nchunk = (a.n + vec - 1) / vec;
+  if (NORM && wide) {
+    // ring of whole rows where every CTA of the persistent grid gets several of them
+    const int nv = a.nchunk <= 1024 ? 2 : 4;
+    const int tpr = ((a.nchunk + nv - 1) / nv + 31) / 32 * 32;
+    const size_t smem = (size_t)kStages * (a.res ? 2 : 1) * a.n * sizeof(T);
+    const int per_sm = (int)(kMaxSmem / (smem + 2048));  // beside static arrays and what the system keeps
+    const int sms = sm_count(), fit = per_sm < 2048 / tpr ? per_sm : 2048 / tpr;
+    if (tpr >= 128 && tpr <= 512 && fit >= 1 && a.rows >= 2LL * sms * fit) {
+      a.tpr = tpr;
+      a.rpc = 1;
+      const int ctas = sms * fit;
+      if (fp8) {
+        if (nv == 2) launch_stream<T, 2, true>(a, ctas, smem, st);
+        else launch_stream<T, 4, true>(a, ctas, smem, st);
+      } else {
+        if (nv == 2) launch_stream<T, 2, false>(a, ctas, smem, st);
+        else launch_stream<T, 4, false>(a, ctas, smem, st);
+      }
+      return cuda_status("rms_norm_quant");
+    }
+  }
   // chunks per thread: few, so that a row's loads are spread over many threads
-  int nv = wide ? 2 : 8;
+  int nv = wide ? 1 : 8;
   while ((a.nchunk + nv - 1) / nv > 1024) nv *= 2;
   a.tpr = ((a.nchunk + nv - 1) / nv + 31) / 32 * 32;
   a.rpc = a.tpr >= 256 ? 1 : 256 / a.tpr;
   if (a.rpc > a.rows) a.rpc = (int)a.rows;
   if (wide) {
     if (fp8) {
-      if (nv == 2) launch<NORM, T, V, 2, true>(a, st);
+      if (nv == 1) launch<NORM, T, V, 1, true>(a, st);
+      else if (nv == 2) launch<NORM, T, V, 2, true>(a, st);
       else launch<NORM, T, V, 4, true>(a, st);
     } else {
-      if (nv == 2) launch<NORM, T, V, 2, false>(a, st);
+      if (nv == 1) launch<NORM, T, V, 1, false>(a, st);
+      else if (nv == 2) launch<NORM, T, V, 2, false>(a, st);
       else launch<NORM, T, V, 4, false>(a, st);
     }
   } else {

@@ -80,6 +80,23 @@ def test_rms_norm_quant(ops, fmt, rows, n, dtype):
     check_quant(plain.q, plain.s, norm_ref(x, w, None)[1], fmt, 32 * U)
 
 
+@pytest.mark.parametrize("fmt,rows,n", [("fp8", 4096, 5120), ("int8", 2047, 1040), ("fp8", 1777, 8192), ("int8", 5000, 4104)])
+def test_rms_norm_quant_many_rows(ops, fmt, rows, n):
+    x, r, w = rnd(1, rows, n, dtype=torch.bfloat16), rnd(2, rows, n, dtype=torch.bfloat16, scale=3.0), 1 + 0.2 * rnd(3, n)
+    x[rows - 1, 3] = float("nan")
+    got = ops.rms_norm_quant(x, w, r, fmt=fmt, normed=True)
+    h, v = norm_ref(x, w, r)
+    last = slice(0, rows - 1)
+    assert torch.equal(got.residual[last].double(), h[last]) and bool(torch.isnan(got.s[rows - 1]).all())
+    within(got.normed[last], v[last], v[last].abs() * (32 * U + BF[torch.bfloat16]))
+    check_quant(got.q[last], got.s[last], v[last], fmt, 32 * U)
+    keep, keep_x = r.clone(), x.clone()
+    again = ops.rms_norm_quant(keep_x, w, keep, fmt=fmt, inplace=True)
+    assert torch.equal(keep[last], got.residual[last]) and torch.equal(again.s[last], got.s[last])
+    one = ops.rms_norm_quant(x[:rows - 1], w, fmt=fmt)
+    check_quant(one.q, one.s, norm_ref(x[last], w, None)[1], fmt, 32 * U)
+
+
 def test_rms_norm_quant_forms(ops):
     x, r, w = rnd(4, 2, 3, 256, dtype=torch.bfloat16), rnd(5, 2, 3, 256, dtype=torch.bfloat16), rnd(6, 256, dtype=torch.bfloat16)
     _, v = norm_ref(x, w, r, 0.1)
