@@ -30,25 +30,40 @@ struct Args {
   void* res_out;      // norm: [rows][n] or null
   void* normed;       // norm: [rows][n] or null
   long long rows;
-  int n, nchunk;      // values per row; chunks of VEC values
+  int n;              // values per row
   int tpr, rpc;       // threads per row (a multiple of 32), rows per CTA
   int w_bf16, pow2;
   float eps, limit;
 };
 
-// A chunk as loaded, and its values: bf16 stays packed in registers until it is used.
-template <typename T, int VEC>
-struct Raw {
-  T v;  // VEC == 1
-  __device__ __forceinline__ void load(const T* p) { v = p[0]; }
-  __device__ __forceinline__ void zero() { v = (T)0.f; }
-  __device__ __forceinline__ void get(float (&o)[VEC]) const { o[0] = (float)v; }
-};
+// VEC values (16 bytes) as loaded; bf16 stays packed in registers until it is used.
+template <typename T>
+struct Raw;
 template <>
-struct Raw<__nv_bfloat16, 8> {
+struct Raw<__nv_bfloat16> {
   uint4 u;
   __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  // the first n values of p alone
+  __device__ __forceinline__ void load_first(const __nv_bfloat16* p, int n) {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) w[i >> 1] |= (uint32_t)h[i] << (16 * (i & 1));
+    u = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // values s.. of this chunk followed by the next one's (0 <= s < 8, the same in every lane of a row)
+  __device__ __forceinline__ void shift_in(const Raw& next, int s) {
+    uint32_t w[8] = {u.x, u.y, u.z, u.w, next.u.x, next.u.y, next.u.z, next.u.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = s & 4 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = s & 2 ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = s & 1 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+    u = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void get(float (&o)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -59,19 +74,48 @@ struct Raw<__nv_bfloat16, 8> {
   }
 };
 template <>
-struct Raw<float, 4> {
+struct Raw<float> {
   float4 u;
   __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
   __device__ __forceinline__ void zero() { u = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load_first(const float* p, int n) {
+    u = make_float4(n > 0 ? p[0] : 0.f, n > 1 ? p[1] : 0.f, n > 2 ? p[2] : 0.f, n > 3 ? p[3] : 0.f);
+  }
+  __device__ __forceinline__ void shift_in(const Raw& next, int s) {
+    float w[8] = {u.x, u.y, u.z, u.w, next.u.x, next.u.y, next.u.z, next.u.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = s & 2 ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = s & 1 ? w[i + 1] : w[i];
+    u = make_float4(w[0], w[1], w[2], w[3]);
+  }
   __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = u.x; o[1] = u.y; o[2] = u.z; o[3] = u.w; }
 };
 
-template <typename T, int VEC>
-__device__ __forceinline__ void store_chunk(T* p, const float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    if constexpr (sizeof(T) == 2) p[0] = __float2bfloat16_rn(v[0]);
-    else p[0] = v[0];
-  } else if constexpr (sizeof(T) == 2) {
+// Chunk at element e (a multiple of VEC) of an array of `total` elements; outside it: zeros. inner: the chunk is
+// known to lie inside (only a tensor's first and last row reach over its ends).
+template <typename T>
+__device__ __forceinline__ Raw<T> load_inside(const T* p, long long e, long long total, bool inner) {
+  constexpr int VEC = 16 / sizeof(T);
+  Raw<T> r;
+  if (inner || (e >= 0 && e + VEC <= total)) r.load(p + e);
+  else if (e >= 0 && e < total) r.load_first(p + e, (int)(total - e));
+  else r.zero();
+  return r;
+}
+// VEC elements from any element e on: two aligned chunks, shifted (s = e mod VEC, the same for a whole row).
+template <typename T>
+__device__ __forceinline__ Raw<T> load_any(const T* p, long long e, long long total, bool inner) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int s = (int)(e & (VEC - 1));
+  Raw<T> r = load_inside(p, e - s, total, inner);
+  if (s) r.shift_in(load_inside(p, e - s + VEC, total, inner), s);
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* p, const float (&v)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -84,30 +128,78 @@ __device__ __forceinline__ void store_chunk(T* p, const float (&v)[VEC]) {
   }
 }
 
+// Where a thread's chunk j lies. Rows of a multiple of VEC values: chunks of the row. Others (EDGE): chunks of
+// the whole array, aligned in memory, of which a row's first and last belong to it in part, so that loads and
+// stores are wide whatever the row length; [lo, hi) are the chunk's values of this row (none: lo = hi = 0).
+struct Span {
+  long long e;  // first element of the chunk in the array
+  int k;        // ... in the row (EDGE: may be negative)
+  int lo, hi;
+};
+template <int VEC, bool EDGE>
+__device__ __forceinline__ Span span_of(const Args& a, long long row, int j, int t, bool live) {
+  Span p;
+  const long long at = row * a.n;
+  if (EDGE) {
+    p.e = (at & ~(long long)(VEC - 1)) + (long long)(j * a.tpr + t) * VEC;
+    p.k = (int)(p.e - at);
+    p.lo = p.k < 0 ? -p.k : 0;
+    p.hi = a.n - p.k < VEC ? a.n - p.k : VEC;
+    if (!live || p.lo >= p.hi) p.lo = p.hi = 0;
+  } else {
+    p.k = (j * a.tpr + t) * VEC;
+    p.e = at + p.k;
+    p.lo = 0;
+    p.hi = live && p.k < a.n ? VEC : 0;
+  }
+  return p;
+}
+template <typename T, bool EDGE>
+__device__ __forceinline__ void store_span(T* p, const Span& s, const float (&v)[16 / sizeof(T)]) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (!EDGE || (s.lo == 0 && s.hi == VEC)) {
+    store_chunk<T>(p + s.e, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i >= s.lo && i < s.hi) p[s.e + i] = (T)v[i];
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ float round_to(float v) {
   if constexpr (sizeof(T) == 2) return __bfloat162float(__float2bfloat16_rn(v));
   else return v;
 }
 
-// weights of VEC consecutive channels, fp32 or bf16
-template <int VEC>
-__device__ __forceinline__ void load_w(const void* w, int w_bf16, int at, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = w_bf16 ? (float)reinterpret_cast<const __nv_bfloat16*>(w)[at] : reinterpret_cast<const float*>(w)[at];
-  } else if (w_bf16) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(reinterpret_cast<const __nv_bfloat16*>(w) + at);
+// weights of VEC consecutive channels from k on, fp32 or bf16; EDGE: any k, zeros outside the row
+template <int VEC, bool EDGE>
+__device__ __forceinline__ void load_w(const Args& a, int k, float (&v)[VEC]) {
+  if (a.w_bf16) {
+    const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(a.w);
+    if constexpr (EDGE) {
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      const uint32_t u = p[i];
-      v[2 * i] = __uint_as_float(u << 16);
-      v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
+      for (int i = 0; i < VEC; ++i) v[i] = k + i >= 0 && k + i < a.n ? (float)w[k + i] : 0.f;
+    } else {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(w + k);
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        const uint32_t u = p[i];
+        v[2 * i] = __uint_as_float(u << 16);
+        v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
+      }
     }
   } else {
+    const float* w = reinterpret_cast<const float*>(a.w);
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
-      const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + at + 4 * i);
-      v[4 * i] = u.x; v[4 * i + 1] = u.y; v[4 * i + 2] = u.z; v[4 * i + 3] = u.w;
+      Raw<float> u;
+      if constexpr (EDGE) u = load_any<float>(w, k + 4 * i, a.n, k >= 8 && k + 16 <= a.n);
+      else u.load(w + k + 4 * i);
+      float f[4];
+      u.get(f);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[4 * i + q] = f[q];
     }
   }
 }
@@ -152,15 +244,12 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr, int 
     if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   if (MAX) top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7FFFFFFFu));
-  if (tpr == 32 && blockDim.x == 32) {
-    __syncwarp();
-    return;
-  }
+  if (tpr == 32) return;  // a row is one warp
   __shared__ float ssums[2][32];  // a second reduction (turn 1) may begin while the first is being read
   __shared__ uint32_t smaxs[2][32];
   float* ssum = ssums[turn];
   uint32_t* smax = smaxs[turn];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = tpr >> 5, w0 = warp / nw * nw;
+  const int lane = threadIdx.x & 31, nw = tpr >> 5, w0 = threadIdx.y * nw, warp = w0 + (threadIdx.x >> 5);
   if (lane == 0) {
     if (SUM) ssum[warp] = sum;
     if (MAX) smax[warp] = __float_as_uint(top);
@@ -175,14 +264,14 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr, int 
 }
 
 // v * mul to 8 bits with its scales; top: the row's max |v| (int8), mul: the row's factor that v still lacks.
-template <int VEC, int NV, bool FP8>
+template <int VEC, int NV, bool FP8, bool EDGE>
 __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][VEC], float mul, float top, long long row,
                                             int t, bool live) {
+  uint8_t* q = reinterpret_cast<uint8_t*>(a.q);
   if constexpr (FP8) {
-    uint8_t* q = reinterpret_cast<uint8_t*>(a.q) + row * a.n;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = j * a.tpr + t;
+      const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
       float m = 0.f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) m = max_nan(m, fabsf(v[j][i]));
@@ -191,117 +280,131 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
       for (int o = 64 / VEC; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float s = scale_of(m * fabsf(mul), 1.0f / 448.0f, a.pow2);
       const float f = mul * __fdividef(1.0f, s);
-      if (live && c < a.nchunk) {
-        if ((c * VEC) % 128 == 0) a.s[row * (a.n / 128) + c * VEC / 128] = s;
+      if (p.hi) {
+        if (p.k % 128 == 0) a.s[row * (a.n / 128) + p.k / 128] = s;
         const uint32_t lo = f32x2_to_e4m3x2(v[j][0] * f, v[j][1] * f) | (f32x2_to_e4m3x2(v[j][2] * f, v[j][3] * f) << 16);
         if constexpr (VEC == 8) {
           const uint32_t hi = f32x2_to_e4m3x2(v[j][4] * f, v[j][5] * f) | (f32x2_to_e4m3x2(v[j][6] * f, v[j][7] * f) << 16);
-          *reinterpret_cast<uint2*>(q + c * VEC) = make_uint2(lo, hi);
+          *reinterpret_cast<uint2*>(q + p.e) = make_uint2(lo, hi);
         } else {
-          *reinterpret_cast<uint32_t*>(q + c * VEC) = lo;
+          *reinterpret_cast<uint32_t*>(q + p.e) = lo;
         }
       }
     }
   } else {
     const float s = scale_of(top * fabsf(mul), 1.0f / 127.0f, 0);
     const float f = mul * __fdividef(1.0f, s);
-    if (!live) return;
-    if (t == 0) a.s[row] = s;
-    uint8_t* q = reinterpret_cast<uint8_t*>(a.q) + row * a.n;
+    if (t == 0 && live) a.s[row] = s;
+    const bool fine = s == s;  // else the row holds a NaN or an infinity: the code 0 throughout
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = j * a.tpr + t;
-      if (c >= a.nchunk) continue;
-      // a row without a scale (NaN or infinity somewhere) has the code 0 throughout
-      auto at = [&](int i) { return s == s ? v[j][i] * f : 0.f; };
-      if constexpr (VEC == 1) {
-        q[c] = (uint8_t)int8x4(at(0), 0.f, 0.f, 0.f);
-      } else if constexpr (VEC == 4) {
-        *reinterpret_cast<uint32_t*>(q + c * VEC) = int8x4(at(0), at(1), at(2), at(3));
+      const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
+      if (!p.hi) continue;
+      uint32_t w[VEC / 4];
+#pragma unroll
+      for (int i = 0; i < VEC / 4; ++i)
+        w[i] = fine ? int8x4(v[j][4 * i] * f, v[j][4 * i + 1] * f, v[j][4 * i + 2] * f, v[j][4 * i + 3] * f) : 0u;
+      if (!EDGE || (p.lo == 0 && p.hi == VEC)) {
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + p.e) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<uint32_t*>(q + p.e) = w[0];
       } else {
-        *reinterpret_cast<uint2*>(q + c * VEC) = make_uint2(int8x4(at(0), at(1), at(2), at(3)),
-                                                            int8x4(at(4), at(5), at(6), at(7)));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i >= p.lo && i < p.hi) q[p.e + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
       }
     }
   }
 }
 
 // One row in registers: residual added and stored, squares and |r w| reduced; v holds r w afterwards.
-template <typename T, int VEC, int NV, bool FP8>
-__device__ __forceinline__ void norm_row(const Args& a, const Raw<T, VEC> (&x)[NV], const Raw<T, VEC> (&r)[NV],
-                                         float (&v)[NV][VEC], float& sum, float& top, long long at, int t, bool live) {
+template <typename T, int NV, bool FP8, bool EDGE>
+__device__ __forceinline__ void norm_row(const Args& a, const Raw<T> (&x)[NV], const Raw<T> (&r)[NV],
+                                         float (&v)[NV][16 / sizeof(T)], float& sum, float& top, long long row, int t, bool live) {
+  constexpr int VEC = 16 / sizeof(T);
   sum = 0.f;
   top = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * a.tpr + t;
+    const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
     x[j].get(v[j]);
-    if (live && c < a.nchunk) {
-      if (a.res) {
-        float y[VEC];
-        r[j].get(y);
+    if (!p.hi) continue;
+    if (a.res) {
+      float y[VEC];
+      r[j].get(y);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = round_to<T>(v[j][i] + y[i]);
-        if (a.res_out) store_chunk<T, VEC>(reinterpret_cast<T*>(a.res_out) + at + c * VEC, v[j]);
-      }
-      float w[VEC];
-      load_w<VEC>(a.w, a.w_bf16, c * VEC, w);
+      for (int i = 0; i < VEC; ++i) v[j][i] = round_to<T>(v[j][i] + y[i]);
+      if (a.res_out) store_span<T, EDGE>(reinterpret_cast<T*>(a.res_out), p, v[j]);
+    }
+    if (EDGE && (p.lo != 0 || p.hi != VEC)) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        sum = fmaf(v[j][i], v[j][i], sum);
-        v[j][i] *= w[i];
-        if (!FP8) top = max_nan(top, fabsf(v[j][i]));
-      }
+      for (int i = 0; i < VEC; ++i)
+        if (i < p.lo || i >= p.hi) v[j][i] = 0.f;  // the neighbouring rows' values
+    }
+    float w[VEC];
+    load_w<VEC, EDGE>(a, p.k, w);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      sum = fmaf(v[j][i], v[j][i], sum);
+      v[j][i] *= w[i];
+      if (!FP8) top = max_nan(top, fabsf(v[j][i]));
     }
   }
 }
 
-template <typename T, int VEC, int NV>
-__device__ __forceinline__ void store_normed(const Args& a, const float (&v)[NV][VEC], float rstd, long long at, int t, bool live) {
-  if (!a.normed || !live) return;
+template <typename T, int NV, bool EDGE>
+__device__ __forceinline__ void store_normed(const Args& a, const float (&v)[NV][16 / sizeof(T)], float rstd, long long row, int t,
+                                             bool live) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (!a.normed) return;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * a.tpr + t;
-    if (c >= a.nchunk) continue;
+    const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
+    if (!p.hi) continue;
     float y[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) y[i] = v[j][i] * rstd;
-    store_chunk<T, VEC>(reinterpret_cast<T*>(a.normed) + at + c * VEC, y);
+    store_span<T, EDGE>(reinterpret_cast<T*>(a.normed), p, y);
   }
 }
 
-template <typename T, int VEC, int NV, bool FP8>
+template <typename T, int NV, bool FP8, bool EDGE>
 __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
-  const int g = threadIdx.x / a.tpr, t = threadIdx.x % a.tpr;
-  const long long row = (long long)blockIdx.x * a.rpc + g;
+  constexpr int VEC = 16 / sizeof(T);
+  const int t = threadIdx.x;
+  const long long row = (long long)blockIdx.x * a.rpc + threadIdx.y, total = a.rows * a.n;
   const bool live = row < a.rows;
-  const long long at = row * a.n;
-  Raw<T, VEC> x[NV], r[NV];
+  Raw<T> x[NV], r[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * a.tpr + t;
+    const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
     x[j].zero();
     r[j].zero();
-    if (live && c < a.nchunk) {
-      x[j].load(reinterpret_cast<const T*>(a.x) + at + c * VEC);
-      if (a.res) r[j].load(reinterpret_cast<const T*>(a.res) + at + c * VEC);
+    if (p.hi) {
+      if constexpr (EDGE) {
+        const bool inner = row + 1 < a.rows;
+        x[j] = load_inside(reinterpret_cast<const T*>(a.x), p.e, total, inner);
+        if (a.res) r[j] = load_inside(reinterpret_cast<const T*>(a.res), p.e, total, inner);
+      } else {
+        x[j].load(reinterpret_cast<const T*>(a.x) + p.e);
+        if (a.res) r[j].load(reinterpret_cast<const T*>(a.res) + p.e);
+      }
     }
   }
-  float v[NV][VEC], sum;
-  float top;
-  norm_row<T, VEC, NV, FP8>(a, x, r, v, sum, top, at, t, live);
+  float v[NV][VEC], sum, top;
+  norm_row<T, NV, FP8, EDGE>(a, x, r, v, sum, top, row, t, live);
   row_reduce<true, !FP8>(sum, top, a.tpr, 0);
   const float rstd = 1.0f / sqrtf(sum / (float)a.n + a.eps);
-  store_normed<T, VEC, NV>(a, v, rstd, at, t, live);
-  quant_store<VEC, NV, FP8>(a, v, rstd, top, row, t, live);
+  store_normed<T, NV, EDGE>(a, v, rstd, row, t, live);
+  quant_store<VEC, NV, FP8, EDGE>(a, v, rstd, top, row, t, live);
 }
 
 // Many rows: a persistent CTA walks rows blockIdx.x + i gridDim.x while bulk copies bring the next ones into a
 // ring of shared memory, so loads stay in flight over the reductions and stores of the rows before.
 constexpr uint64_t kWaitNs = 1000000000ull;
 
-template <typename T, int VEC, int NV, bool FP8>
+template <typename T, int NV, bool FP8>
 __global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
+  constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ uint64_t full[kStages];
   const int t = threadIdx.x, terms = a.res ? 2 : 1;
@@ -326,31 +429,30 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
     const int s = i % kStages;
     const bool ok = mbar_wait(&full[s], (i / kStages) & 1, kWaitNs);
     const T* st = reinterpret_cast<const T*>(sm + (size_t)s * terms * row_bytes);
-    Raw<T, VEC> x[NV], r[NV];
+    Raw<T> x[NV], r[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = j * a.tpr + t;
       x[j].zero();
       r[j].zero();
-      if (c < a.nchunk) {
+      if (c * VEC < a.n) {
         x[j].load(st + c * VEC);
         if (a.res) r[j].load(st + a.n + c * VEC);
       }
     }
-    float v[NV][VEC], sum;
-    float top;
-    norm_row<T, VEC, NV, FP8>(a, x, r, v, sum, top, row * a.n, t, true);
+    float v[NV][VEC], sum, top;
+    norm_row<T, NV, FP8, false>(a, x, r, v, sum, top, row, t, true);
     row_reduce<true, !FP8>(sum, top, a.tpr, i & 1);  // its barrier: every thread has read the stage
     if (t == 0 && row + kStages * step < a.rows) fetch(row + kStages * step, s);
     // an expired wait leaves a row of NaN
     const float rstd = ok ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : __int_as_float(0x7FC00000);
-    store_normed<T, VEC, NV>(a, v, rstd, row * a.n, t, true);
-    quant_store<VEC, NV, FP8>(a, v, rstd, top, row, t, true);
+    store_normed<T, NV, false>(a, v, rstd, row, t, true);
+    quant_store<VEC, NV, FP8, false>(a, v, rstd, top, row, t, true);
   }
 }
 
-// silu(g) u with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + d ln 2) with t = -g log2(e) rounded and d what the
-// rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all that is
+// silu(g) u with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + r) with t = -g log2(e) rounded and r = -g - t ln 2,
+// what the rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all that is
 // approximated; the argument's own rounding would cost |g| units. exp's argument stops at 87, where silu(g) is
 // below 1e-35, so that the reciprocal stays a normal number.
 __device__ __forceinline__ float swiglu(float g, float u, float limit) {
@@ -358,46 +460,60 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
   u = max_nan(min_nan(u, limit), -limit);
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
   const float a = max_nan(g, -87.0f);
-  const float t = -a * kLog2e, d = fmaf(-a, kLog2e, -t);
+  const float t = a * -kLog2e, d = fmaf(t, -kLn2, -a);
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  e = 1.0f + fmaf(e, d * kLn2, e);
+  e = 1.0f + fmaf(e, d, e);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
   return g * r * u;
 }
 
-template <typename T, int VEC, int NV, bool FP8>
+template <typename T, int NV, bool FP8, bool EDGE>
 __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
-  const int gidx = threadIdx.x / a.tpr, t = threadIdx.x % a.tpr;
-  const long long row = (long long)blockIdx.x * a.rpc + gidx;
+  constexpr int VEC = 16 / sizeof(T);
+  const int t = threadIdx.x;
+  const long long row = (long long)blockIdx.x * a.rpc + threadIdx.y, total = 2 * a.rows * a.n;
   const bool live = row < a.rows;
-  const T* g = reinterpret_cast<const T*>(a.x) + row * 2 * a.n;
-  Raw<T, VEC> x[NV], y[NV];
+  const T* gu = reinterpret_cast<const T*>(a.x);
+  Raw<T> x[NV], y[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int c = j * a.tpr + t;
+    const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
+    const long long e = 2 * row * a.n + p.k;
     x[j].zero();
     y[j].zero();
-    if (live && c < a.nchunk) {
-      x[j].load(g + c * VEC);
-      y[j].load(g + a.n + c * VEC);
+    if (p.hi) {
+      if constexpr (EDGE) {  // the codes' chunks are aligned; g and u lie at their own offsets to them
+        const bool inner = row > 0 && row + 1 < a.rows;
+        x[j] = load_any(gu, e, total, inner);
+        y[j] = load_any(gu, e + a.n, total, inner);
+      } else {
+        x[j].load(gu + e);
+        y[j].load(gu + e + a.n);
+      }
     }
   }
   const float wr = live && a.w ? reinterpret_cast<const float*>(a.w)[row] : 1.0f;
   float v[NV][VEC], top = 0.f, none = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
+    const Span p = span_of<VEC, EDGE>(a, row, j, t, live);
     float u[VEC];
     x[j].get(v[j]);
     y[j].get(u);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[j][i] = swiglu(v[j][i], u[i], a.limit);
-      if (!FP8) top = max_nan(top, fabsf(v[j][i]));
+    for (int i = 0; i < VEC; ++i) v[j][i] = swiglu(v[j][i], u[i], a.limit);
+    if (EDGE && (p.lo != 0 || p.hi != VEC)) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (i < p.lo || i >= p.hi) v[j][i] = 0.f;  // the neighbouring rows' values
     }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (!FP8) top = max_nan(top, fabsf(v[j][i]));
   }
   if (!FP8) row_reduce<false, true>(none, top, a.tpr, 0);
-  quant_store<VEC, NV, FP8>(a, v, wr, top, row, t, live);
+  quant_store<VEC, NV, FP8, EDGE>(a, v, wr, top, row, t, live);
 }
 
 int sm_count() {
@@ -407,30 +523,36 @@ int sm_count() {
   return sms;
 }
 
-template <bool NORM, typename T, int VEC, int NV, bool FP8>
+template <bool NORM, typename T, int NV, bool FP8, bool EDGE>
 void launch(const Args& a, cudaStream_t st) {
   const long long grid = (a.rows + a.rpc - 1) / a.rpc;
-  if (NORM) norm_kernel<T, VEC, NV, FP8><<<(unsigned)grid, a.tpr * a.rpc, 0, st>>>(a);
-  else swiglu_kernel<T, VEC, NV, FP8><<<(unsigned)grid, a.tpr * a.rpc, 0, st>>>(a);
+  if (NORM) norm_kernel<T, NV, FP8, EDGE><<<(unsigned)grid, dim3(a.tpr, a.rpc), 0, st>>>(a);
+  else swiglu_kernel<T, NV, FP8, EDGE><<<(unsigned)grid, dim3(a.tpr, a.rpc), 0, st>>>(a);
+}
+template <bool NORM, typename T, bool FP8, bool EDGE>
+void launch_nv(const Args& a, int nv, cudaStream_t st) {
+  if (nv == 1) launch<NORM, T, 1, FP8, EDGE>(a, st);
+  else if (nv == 2) launch<NORM, T, 2, FP8, EDGE>(a, st);
+  else if (nv == 4) launch<NORM, T, 4, FP8, EDGE>(a, st);
+  else if constexpr (EDGE && sizeof(T) == 4) launch<NORM, T, 8, FP8, EDGE>(a, st);  // the longest: 4097 chunks
 }
 
 template <typename T, int NV, bool FP8>
 void launch_stream(const Args& a, int ctas, size_t smem, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  auto k = norm_stream_kernel<T, V, NV, FP8>;
+  auto k = norm_stream_kernel<T, NV, FP8>;
   if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   k<<<ctas, a.tpr, smem, st>>>(a);
 }
 
 template <bool NORM, typename T>
-int run(Args& a, bool fp8, bool wide, cudaStream_t st) {
+int run(Args& a, bool fp8, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const int vec = wide ? V : 1;
-  a.nchunk = (a.n + vec - 1) / vec;
-  if (NORM && wide) {
+  const bool edge = a.n % V != 0;
+  const int nchunk = edge ? (a.n - 2) / V + 2 : a.n / V;  // a row's chunks, at most
+  if (NORM && !edge) {
     // ring of whole rows where every CTA of the persistent grid gets several of them
-    const int nv = a.nchunk <= 1024 ? 2 : 4;
-    const int tpr = ((a.nchunk + nv - 1) / nv + 31) / 32 * 32;
+    const int nv = nchunk <= 1024 ? 2 : 4;
+    const int tpr = ((nchunk + nv - 1) / nv + 31) / 32 * 32;
     const size_t smem = (size_t)kStages * (a.res ? 2 : 1) * a.n * sizeof(T);
     const int per_sm = (int)(kMaxSmem / (smem + 2048));  // beside static arrays and what the system keeps
     const int sms = sm_count(), fit = per_sm < 2048 / tpr ? per_sm : 2048 / tpr;
@@ -448,26 +570,20 @@ int run(Args& a, bool fp8, bool wide, cudaStream_t st) {
       return cuda_status("rms_norm_quant");
     }
   }
-  // chunks per thread: few, so that a row's loads are spread over many threads
-  int nv = wide ? 1 : 8;
-  while ((a.nchunk + nv - 1) / nv > 1024) nv *= 2;
-  a.tpr = ((a.nchunk + nv - 1) / nv + 31) / 32 * 32;
+  // Chunks per thread: one while there are few rows (a row's loads at once over many threads: 300 rows of 2048
+  // int8 codes 2.6 us, 2.9 with four), up to four where the grid fills the GPU and a thread's fixed instructions
+  // count (12282 rows 26.8 us, 33.2 with one). A row keeps its 32 threads. With an edge one chunk is as fast as
+  // two (6000 rows of 2049 24.9 us, 26.8).
+  int nv = 1;
+  while ((nchunk + nv - 1) / nv > 1024) nv *= 2;
+  if (!edge && a.rows * nchunk >= 8192LL * sm_count())
+    while (nv < 4 && nchunk >= 64 * nv) nv *= 2;
+  a.tpr = ((nchunk + nv - 1) / nv + 31) / 32 * 32;
   a.rpc = a.tpr >= 256 ? 1 : 256 / a.tpr;
   if (a.rpc > a.rows) a.rpc = (int)a.rows;
-  if (wide) {
-    if (fp8) {
-      if (nv == 1) launch<NORM, T, V, 1, true>(a, st);
-      else if (nv == 2) launch<NORM, T, V, 2, true>(a, st);
-      else launch<NORM, T, V, 4, true>(a, st);
-    } else {
-      if (nv == 1) launch<NORM, T, V, 1, false>(a, st);
-      else if (nv == 2) launch<NORM, T, V, 2, false>(a, st);
-      else launch<NORM, T, V, 4, false>(a, st);
-    }
-  } else {
-    if (nv == 8) launch<NORM, T, 1, 8, false>(a, st);
-    else launch<NORM, T, 1, 16, false>(a, st);
-  }
+  if (fp8) launch_nv<NORM, T, true, false>(a, nv, st);
+  else if (edge) launch_nv<NORM, T, false, true>(a, nv, st);
+  else launch_nv<NORM, T, false, false>(a, nv, st);
   return cuda_status(NORM ? "rms_norm_quant" : "swiglu_quant");
 }
 
@@ -511,18 +627,15 @@ extern "C" int dsmoe_rms_norm_quant(const void* x, int dtype, const void* residu
                     !rows8::overlap(q, rows * hidden, residual, nb) && !rows8::overlap(q, rows * hidden, residual_out, nb) &&
                     !rows8::overlap(q, rows * hidden, normed, nb),
                 DSMOE_ERR_ARG, "rms_norm_quant: outputs overlap inputs");
-  const uintptr_t any = (uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)residual_out | (uintptr_t)normed;
-  DSMOE_REQUIRE((any & (sz - 1)) == 0 && ((uintptr_t)s & 3) == 0 &&
-                    ((uintptr_t)weight & (w_dtype == DSMOE_DTYPE_F32 ? 3 : 1)) == 0,
+  DSMOE_REQUIRE((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)residual_out | (uintptr_t)normed |
+                  (uintptr_t)q) & 15) == 0 && ((uintptr_t)s & 3) == 0,
                 DSMOE_ERR_ALIGN, "rms_norm_quant: misaligned pointer");
-  const bool wide = (any & 15) == 0 && ((uintptr_t)q & 7) == 0 && hidden * sz % 16 == 0;
-  DSMOE_REQUIRE(wide || q_dtype == DSMOE_DTYPE_I8, DSMOE_ERR_ALIGN, "rms_norm_quant: e4m3 rows need 16-byte aligned pointers");
   rows8::Args a{};
   a.x = x; a.res = residual; a.w = weight; a.q = q; a.s = s; a.res_out = residual_out; a.normed = normed;
   a.rows = rows; a.n = (int)hidden; a.w_bf16 = w_dtype == DSMOE_DTYPE_BF16; a.pow2 = pow2; a.eps = eps;
   const bool fp8 = q_dtype == DSMOE_DTYPE_E4M3;
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == DSMOE_DTYPE_F32 ? rows8::run<true, float>(a, fp8, wide, st) : rows8::run<true, __nv_bfloat16>(a, fp8, wide, st);
+  return dtype == DSMOE_DTYPE_F32 ? rows8::run<true, float>(a, fp8, st) : rows8::run<true, __nv_bfloat16>(a, fp8, st);
 }
 
 extern "C" int dsmoe_swiglu_quant(const void* gu, int dtype, const float* row_weight, long long rows, long long inter,
@@ -532,14 +645,12 @@ extern "C" int dsmoe_swiglu_quant(const void* gu, int dtype, const float* row_we
   DSMOE_REQUIRE(gu, DSMOE_ERR_ARG, "swiglu_quant: null pointer");
   DSMOE_REQUIRE(limit > 0.f, DSMOE_ERR_ARG, "swiglu_quant: limit must be positive");
   const int sz = dtype == DSMOE_DTYPE_F32 ? 4 : 2;
-  DSMOE_REQUIRE(((uintptr_t)gu & (sz - 1)) == 0 && (((uintptr_t)s | (uintptr_t)row_weight) & 3) == 0, DSMOE_ERR_ALIGN,
+  DSMOE_REQUIRE((((uintptr_t)gu | (uintptr_t)q) & 15) == 0 && (((uintptr_t)s | (uintptr_t)row_weight) & 3) == 0, DSMOE_ERR_ALIGN,
                 "swiglu_quant: misaligned pointer");
   DSMOE_REQUIRE(!rows8::overlap(q, rows * inter, gu, 2 * rows * inter * sz), DSMOE_ERR_ARG, "swiglu_quant: q overlaps gu");
-  const bool wide = ((uintptr_t)gu & 15) == 0 && ((uintptr_t)q & 7) == 0 && inter * sz % 16 == 0;
-  DSMOE_REQUIRE(wide || q_dtype == DSMOE_DTYPE_I8, DSMOE_ERR_ALIGN, "swiglu_quant: e4m3 rows need 16-byte aligned pointers");
   rows8::Args a{};
   a.x = gu; a.w = row_weight; a.q = q; a.s = s; a.rows = rows; a.n = (int)inter; a.pow2 = pow2; a.limit = limit;
   const bool fp8 = q_dtype == DSMOE_DTYPE_E4M3;
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == DSMOE_DTYPE_F32 ? rows8::run<false, float>(a, fp8, wide, st) : rows8::run<false, __nv_bfloat16>(a, fp8, wide, st);
+  return dtype == DSMOE_DTYPE_F32 ? rows8::run<false, float>(a, fp8, st) : rows8::run<false, __nv_bfloat16>(a, fp8, st);
 }

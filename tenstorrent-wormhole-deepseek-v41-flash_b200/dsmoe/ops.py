@@ -138,20 +138,20 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional[tor
         _want(name, residual, "residual", x.dtype, x.shape)
     if inplace and (residual is None or not residual.is_contiguous()):
         raise ValueError(f"{name}: inplace needs a contiguous residual")
-    if inplace and fmt == "fp8" and residual.data_ptr() % 16:
-        raise ValueError(f"{name}: inplace with fmt 'fp8' needs a 16-byte aligned residual")
     code, q, s = _quant_out(name, fmt, scale_fmt, x, h)
     x, weight = _dense(x), _dense(weight)
-    out = None
+    out = keep = None
     if residual is not None:
-        residual = residual if inplace else _dense(residual)
+        keep, residual = residual, _dense(residual)
         out = residual if inplace else torch.empty_like(residual)
     y = torch.empty_like(x) if normed else None
     if x.numel():
         _call(L.lib.dsmoe_rms_norm_quant, x, x.data_ptr(), _FLOATS[x.dtype], L.ptr(residual), weight.data_ptr(),
               _FLOATS[weight.dtype], x.numel() // h, h, eps, code, 1 if scale_fmt is not None else 0, q.data_ptr(),
               s.data_ptr(), L.ptr(out), L.ptr(y))
-    return NormQuant(q, s, out, y)
+        if inplace and out is not keep and out.data_ptr() != keep.data_ptr():  # it was not 16-byte aligned
+            keep.copy_(out)
+    return NormQuant(q, s, keep if inplace else out, y)
 
 
 def swiglu_quant(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, *, limit: float = 10.0, fmt: str = "int8",

@@ -63,7 +63,7 @@ def norm_ref(x, w, r, eps=1e-6):
 
 NORM_SHAPES = [("fp8", 1, 128), ("fp8", 1, 5120), ("fp8", 3, 1024), ("fp8", 33, 2304), ("fp8", 150, 8192), ("fp8", 5, 16384),
                ("int8", 1, 1), ("int8", 2, 7), ("int8", 1, 5120), ("int8", 65, 1040), ("int8", 9, 8191), ("int8", 4, 16384),
-               ("int8", 5, 12345), ("int8", 301, 257), ("int8", 7, 4098)]
+               ("int8", 5, 12345), ("int8", 301, 257), ("int8", 7, 4098), ("int8", 9, 16383), ("int8", 40, 9), ("int8", 33, 2)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -118,8 +118,9 @@ def test_rms_norm_quant_forms(ops):
     odd = torch.cat([r.new_zeros(1), r.flatten()])[1:].view(2, 3, 256)  # in place at an odd address
     i8, want = ops.rms_norm_quant(x, w, odd, fmt="int8", inplace=True), ops.rms_norm_quant(x, w, r, fmt="int8")
     assert torch.equal(odd, want.residual) and torch.equal(i8.q, want.q)
-    with pytest.raises(ValueError):
-        ops.rms_norm_quant(x, w, torch.cat([r.new_zeros(1), r.flatten()])[1:].view(2, 3, 256), inplace=True)
+    odd = torch.cat([r.new_zeros(1), r.flatten()])[1:].view(2, 3, 256)
+    f8 = ops.rms_norm_quant(x, w, odd, eps=0.1, inplace=True)
+    assert f8.residual is odd and torch.equal(odd, got.residual) and torch.equal(f8.s, got.s)
     # one tensor as both terms
     twice = ops.rms_norm_quant(x, w, x, fmt="int8")
     check_quant(twice.q, twice.s, norm_ref(x, w, x)[1], "int8", 32 * U)
@@ -154,7 +155,8 @@ def swiglu_ref(gu, wr=None, limit=10.0):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fmt,rows,n", [("fp8", 1, 128), ("fp8", 48, 2048), ("fp8", 5, 2304), ("fp8", 3, 16384), ("int8", 1, 1),
                                         ("int8", 3, 7), ("int8", 48, 2048), ("int8", 5, 2049), ("int8", 200, 288),
-                                        ("int8", 3, 16384), ("int8", 2, 9001)])
+                                        ("int8", 3, 16384), ("int8", 2, 9001), ("int8", 9, 16383), ("int8", 70, 5), ("int8", 33, 130),
+                                        ("int8", 17, 1027)])
 def test_swiglu_quant(ops, fmt, rows, n, dtype):
     gu, wr = rnd(8, rows, 2 * n, dtype=dtype, scale=4.0), rnd(9, rows).abs() + 0.1
     q, s = ops.swiglu_quant(gu, fmt=fmt)
