@@ -8,6 +8,8 @@
 // offsets[E] hold zeros.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace dsmoe {
@@ -19,58 +21,78 @@ constexpr int kMaxExperts = 1024;
 constexpr int kMaxTopk = 64;
 
 // ------------------------------------------------------------------ sort
-// One cluster of C CTAs (C = 1 for few pairs). Warp w of CTA c owns a contiguous run of pairs and a
-// row of counters in shared memory. Count; prefix over the warps of the CTA, the CTAs of the cluster
-// (their totals read through distributed shared memory) and the experts; then each warp walks its run
-// again, 32 pairs at a time, and ranks equal experts among its lanes by match.
+// One cluster of C CTAs (C = 1 for few pairs). Counting warp w of CTA c owns a contiguous run of pairs and a
+// row of counters in shared memory. Count; prefix over the warps of the CTA, the CTAs of the cluster (their
+// totals read through distributed shared memory) and the experts; then each warp walks its run again, 32
+// pairs at a time, and ranks equal experts among its lanes by match. Bound by latency: a launch, two reads of
+// idx, a cluster barrier and the scan; loads are issued kBatch at a time.
 struct SortArgs {
   const int64_t* idx;
   int* pos;
   int* src;
   int* offsets;
   int n, E;
-  int run;  // pairs per warp, a multiple of 32
+  int run, cw;  // pairs per counting warp (a multiple of 32), counting warps of a CTA
 };
+constexpr int kBatch = 4;
+constexpr int kSortSmem = (34 * kMaxExperts + 32) * (int)sizeof(int);  // at most
 
+template <int C>
 __global__ void __launch_bounds__(1024) sort_kernel(const SortArgs a) {
   extern __shared__ int sm[];
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = cluster.num_blocks(), rank = cluster.block_rank();
+  const int rank = C > 1 ? (int)cluster.block_rank() : 0;
   const int nt = blockDim.x, tid = threadIdx.x, nw = nt >> 5, warp = tid >> 5, lane = tid & 31;
-  int* hist = sm;               // [nw][E]
-  int* total = hist + nw * a.E; // [E] pairs of each expert in this CTA
-  int* off = total + a.E;       // [E] first row of each expert, then of this CTA's pairs of it
-  int* part = off + a.E;        // [32] warp sums of the scan
-  for (int i = tid; i < nw * a.E; i += nt) hist[i] = 0;
+  int* hist = sm;                 // [cw][E]
+  int* total = hist + a.cw * a.E; // [E] pairs of each expert in this CTA
+  int* off = total + a.E;         // [E] first row of this CTA's pairs of each expert
+  int* part = off + a.E;          // [32] warp sums of the scan
+  long long first = (long long)(rank * a.cw + warp) * a.run;
+  if (warp >= a.cw || first > a.n) first = a.n;
+  const int lo = (int)first, hi = warp < a.cw && first + a.run < a.n ? (int)(first + a.run) : a.n;
+  // the pairs from i0 on, -1 where there is none or its expert is outside
+  auto keys = [&](int i0, int (&key)[kBatch]) {
+    long long e[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) e[q] = i0 + 32 * q + lane < hi ? a.idx[i0 + 32 * q + lane] : -1;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) key[q] = e[q] >= 0 && e[q] < a.E ? (int)e[q] : -1;
+  };
+  int key[kBatch];
+  if (lo < hi) keys(lo, key);
+  for (int i = tid; i < a.cw * a.E; i += nt) hist[i] = 0;
   __syncthreads();
   int* mine = hist + warp * a.E;
-  const long long first = (long long)(rank * nw + warp) * a.run;
-  const int lo = first < a.n ? (int)first : a.n, hi = first + a.run < a.n ? (int)(first + a.run) : a.n;
-  for (int i = lo + lane; i < hi; i += 32) {
-    const long long e = a.idx[i];
-    if (e >= 0 && e < a.E) atomicAdd(&mine[e], 1);
+  for (int i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    if (i0 > lo) keys(i0, key);
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+      if (key[q] >= 0) atomicAdd(&mine[key[q]], 1);
   }
   __syncthreads();
   for (int e = tid; e < a.E; e += nt) {
     int sum = 0;
-    for (int w = 0; w < nw; ++w) {
+    for (int w = 0; w < a.cw; ++w) {
       const int c = hist[w * a.E + e];
       hist[w * a.E + e] = sum;
       sum += c;
     }
     total[e] = sum;
   }
-  cluster.sync();
+  if (C > 1) cluster.sync();
   // exclusive prefix over the experts of the whole cluster's counts, nt experts at a time
   int carry = 0;
   for (int e0 = 0; e0 < a.E; e0 += nt) {
     const int e = e0 + tid;
     int before = 0, all = 0;
     if (e < a.E) {
+      int v[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c] = C == 1 ? total[e] : cluster.map_shared_rank(total, c)[e];
+#pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int v = C == 1 ? total[e] : cluster.map_shared_rank(total, c)[e];
-        if (c < rank) before += v;
-        all += v;
+        if (c < rank) before += v[c];
+        all += v[c];
       }
     }
     int inc = all;
@@ -81,41 +103,48 @@ __global__ void __launch_bounds__(1024) sort_kernel(const SortArgs a) {
     }
     if (lane == 31) part[warp] = inc;
     __syncthreads();
-    int below = carry, sum = 0;
-    for (int w = 0; w < nw; ++w) {
-      if (w < warp) below += part[w];
-      sum += part[w];
+    int p = lane < nw ? part[lane] : 0;  // every warp scans the warps' sums
+    const int own = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, p, o);
+      if (lane >= o) p += v;
     }
-    __syncthreads();
+    const int start = carry + __shfl_sync(0xffffffffu, p - own, warp) + inc - all;
+    carry += __shfl_sync(0xffffffffu, p, 31);
     if (e < a.E) {
-      const int start = below + inc - all;
       off[e] = start + before;
       if (rank == 0) a.offsets[e] = start;
     }
-    carry += sum;
+    __syncthreads();
   }
   if (rank == 0 && tid == 0) a.offsets[a.E] = carry;
-  __syncthreads();
-  for (int i0 = lo; i0 < hi; i0 += 32) {
-    const int i = i0 + lane;
-    long long e = -1;
-    if (i < hi) e = a.idx[i];
-    const bool ok = e >= 0 && e < a.E;
-    const int key = ok ? (int)e : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, key);
-    int p = -1;
-    if (ok) p = off[key] + mine[key] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (ok && (same >> lane) == 1u) mine[key] += __popc(same);  // the last lane of each expert
-    __syncwarp();
-    if (i < hi) {
-      a.pos[i] = p;
-      if (ok) a.src[p] = i;
+  if (hi - lo > 32 * kBatch) keys(lo, key);
+  for (int i0 = lo; i0 < hi; i0 += 32 * kBatch) {
+    int next[kBatch];
+    if (i0 + 32 * kBatch < hi) keys(i0 + 32 * kBatch, next);
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + 32 * q + lane;
+      if (i0 + 32 * q >= hi) break;
+      const unsigned same = __match_any_sync(0xffffffffu, key[q]);
+      const bool ok = key[q] >= 0;
+      int p = -1;
+      if (ok) p = off[key[q]] + mine[key[q]] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (ok && (same >> lane) == 1u) mine[key[q]] += __popc(same);  // the last lane of each expert
+      __syncwarp();
+      if (i < hi) {
+        a.pos[i] = p;
+        if (ok) a.src[p] = i;
+      }
     }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) key[q] = next[q];
   }
   // rows behind the last pair
   for (int i = carry + rank * nt + tid; i < a.n; i += C * nt) a.src[i] = -1;
-  cluster.sync();  // no CTA leaves while another may still read its totals
+  if (C > 1) cluster.sync();  // no CTA leaves while another may still read its totals
 }
 
 // ------------------------------------------------------------------ rows
@@ -149,23 +178,33 @@ __global__ void dispatch_kernel(const U* __restrict__ x, const float* __restrict
   if (ss && blockIdx.y == 0 && threadIdx.x < k && place[threadIdx.x] >= 0) ss[place[threadIdx.x]] = s[t];
 }
 
+// VEC values of a row as loaded (16 bytes, or one value where the row or an address is not a multiple of 16
+// bytes): they stay packed until they are used, which keeps registers few and warps many.
 template <typename T, int VEC>
-__device__ __forceinline__ void load_row(const T* p, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = (float)p[0];
-  } else if constexpr (sizeof(T) == 2) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+struct Raw {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = p[0]; }
+  __device__ __forceinline__ void get(float (&o)[VEC]) const { o[0] = (float)v; }
+};
+template <>
+struct Raw<__nv_bfloat16, 8> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&o)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      o[2 * i] = __uint_as_float(w[i] << 16);
+      o[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
-  } else {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
   }
-}
+};
+template <>
+struct Raw<float, 4> {
+  float4 u;
+  __device__ __forceinline__ void load(const float* p) { u = *reinterpret_cast<const float4*>(p); }
+  __device__ __forceinline__ void get(float (&o)[4]) const { o[0] = u.x; o[1] = u.y; o[2] = u.z; o[3] = u.w; }
+};
 
 template <typename T, int VEC>
 __device__ __forceinline__ void store_row(T* p, const float (&v)[VEC]) {
@@ -185,8 +224,9 @@ __device__ __forceinline__ void store_row(T* p, const float (&v)[VEC]) {
 }
 
 // y[t] in fp32, choices added in order j, rounded once.
+constexpr int kRows = 4;
 template <typename T, int VEC>
-__global__ void combine_kernel(const T* __restrict__ ys, const int* __restrict__ pos, const float* __restrict__ wt, int k, int n,
+__global__ void __launch_bounds__(256, 7) combine_kernel(const T* __restrict__ ys, const int* __restrict__ pos, const float* __restrict__ wt, int k, int n,
                                long long width, T* __restrict__ y) {
   const long long t = blockIdx.x;
   __shared__ int place[kMaxTopk];
@@ -202,67 +242,93 @@ __global__ void combine_kernel(const T* __restrict__ ys, const int* __restrict__
     float acc[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
-    for (int j = 0; j < k; ++j) {
-      if (place[j] < 0) continue;
-      float v[VEC];
-      load_row<T, VEC>(ys + place[j] * width + c, v);
+    for (int j0 = 0; j0 < k; j0 += kRows) {  // loads of kRows choices at once
+      Raw<T, VEC> raw[kRows];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = fmaf(weight[j], v[i], acc[i]);
+      for (int q = 0; q < kRows; ++q) {
+        const int p = j0 + q < k ? place[j0 + q] : -1;
+        if (p >= 0) raw[q].load(ys + p * width + c);
+      }
+#pragma unroll
+      for (int q = 0; q < kRows; ++q) {
+        if (j0 + q >= k || place[j0 + q] < 0) continue;
+        float v[VEC];
+        raw[q].get(v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(weight[j0 + q], v[i], acc[i]);
+      }
     }
     store_row<T, VEC>(y + t * width + c, acc);
   }
 }
 
-// One CTA per token; dwt's dot products are summed lane, warp, block, in a fixed order.
+// One CTA for kRows choices of a token: its dy row is read once for them, their rows of ys are read, their rows
+// of dys written, and dwt's dot products summed lane, warp, block, in a fixed order.
 template <typename T, int VEC>
-__global__ void combine_grad_kernel(const T* __restrict__ dy, const T* __restrict__ ys, const int* __restrict__ pos,
-                                    const float* __restrict__ wt, const int* __restrict__ offsets, int E, int k, int n,
-                                    long long width, T* __restrict__ dys, float* __restrict__ dwt) {
-  const long long t = blockIdx.x;
-  __shared__ int place[kMaxTopk];
-  __shared__ float weight[kMaxTopk];
-  __shared__ float part[32];
-  if (threadIdx.x < k) {
-    const int p = pos[t * k + threadIdx.x];
-    place[threadIdx.x] = p >= 0 && p < n ? p : -1;
-    weight[threadIdx.x] = wt ? wt[t * k + threadIdx.x] : 1.0f;
-  }
-  __syncthreads();
+__global__ void __launch_bounds__(256, 6) combine_grad_kernel(const T* __restrict__ dy, const T* __restrict__ ys,
+                                                              const int* __restrict__ pos, const float* __restrict__ wt,
+                                                              const int* __restrict__ offsets, int E, int k, int n,
+                                                              long long width, T* __restrict__ dys, float* __restrict__ dwt) {
+  const int batches = (k + kRows - 1) / kRows;
+  const long long t = blockIdx.x / batches;
+  const int j0 = blockIdx.x % batches * kRows;
+  __shared__ float part[kRows][32];
   const int live = min(max(offsets[E], 0), n);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  for (int j = 0; j < k; ++j) {
-    const int p = place[j];
-    float sum = 0.f;
-    if (p >= 0) {
-      for (long long c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) {
-        float g[VEC], v[VEC];
-        load_row<T, VEC>(dy + t * width + c, g);
-        if (dwt) {
-          load_row<T, VEC>(ys + p * width + c, v);
+  int place[kRows];
+  float w[kRows], sum[kRows];
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) sum = fmaf(g[i], v[i], sum);
-        }
-        if (dys) {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[i] = g[i] * weight[j];
-          store_row<T, VEC>(dys + p * width + c, v);
-        }
-      }
-    }
+  for (int q = 0; q < kRows; ++q) {
+    const long long r = t * k + j0 + q;
+    const int p = j0 + q < k ? pos[r] : -1;
+    place[q] = p >= 0 && p < n ? p : -1;
+    w[q] = wt && place[q] >= 0 ? wt[r] : 1.0f;
+    sum[q] = 0.f;
+  }
+  for (long long c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) {
+    Raw<T, VEC> rg, rv[kRows];
+    rg.load(dy + t * width + c);
     if (dwt) {
-      sum = warp_sum(sum);
-      if (lane == 0) part[warp] = sum;
-      __syncthreads();
-      if (warp == 0) {
-        sum = warp_sum(lane < nw ? part[lane] : 0.f);
-        if (lane == 0) dwt[t * k + j] = sum;
-      }
-      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kRows; ++q)
+        if (place[q] >= 0) rv[q].load(ys + place[q] * width + c);
     }
-    const long long r = t * k + j;
-    if (dys && r >= live) {
+    float g[VEC];
+    rg.get(g);
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      if (place[q] < 0) continue;
+      float v[VEC];
+      if (dwt) {
+        rv[q].get(v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[q] = fmaf(g[i], v[i], sum[q]);
+      }
+      if (dys) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = g[i] * w[q];
+        store_row<T, VEC>(dys + place[q] * width + c, v);
+      }
+    }
+  }
+  if (dys) {
+    for (int q = 0; q < kRows && j0 + q < k; ++q) {
+      const long long r = t * k + j0 + q;
+      if (r < live) continue;  // else this choice's number is that of a row behind the last
       const float zero[VEC] = {};
       for (long long c = threadIdx.x * VEC; c < width; c += blockDim.x * VEC) store_row<T, VEC>(dys + r * width + c, zero);
+    }
+  }
+  if (dwt) {
+#pragma unroll
+    for (int q = 0; q < kRows; ++q) {
+      sum[q] = warp_sum(sum[q]);
+      if (lane == 0) part[q][warp] = sum[q];
+    }
+    __syncthreads();
+    if (warp < kRows && j0 + warp < k) {
+      const float s = warp_sum(lane < nw ? part[warp][lane] : 0.f);
+      if (lane == 0) dwt[t * k + j0 + warp] = s;
     }
   }
 }
@@ -321,13 +387,41 @@ void combine_grad(const void* dy, const void* ys, const int* pos, const float* w
                   long long width, bool wide, void* dys, float* dwt, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   int th = threads_for(wide ? width / V : width);
-  if (th < k) th = 64;
+  if (th < 32 * kRows) th = 32 * kRows;  // a warp joins each choice's sums
+  const int n = (int)(P * k), grid = (int)(P * ((k + kRows - 1) / kRows));
   if (wide)
-    combine_grad_kernel<T, V><<<(unsigned)P, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, (int)(P * k), width,
-                                                          (T*)dys, dwt);
+    combine_grad_kernel<T, V><<<grid, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, n, width, (T*)dys, dwt);
   else
-    combine_grad_kernel<T, 1><<<(unsigned)P, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, (int)(P * k), width,
-                                                          (T*)dys, dwt);
+    combine_grad_kernel<T, 1><<<grid, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, n, width, (T*)dys, dwt);
+}
+
+// Whether the current device runs clusters of 16 CTAs (more than 8 is not portable); asked once per device.
+bool sixteen() {
+  static std::atomic<int> known[64];  // 0 unknown, 1 yes, 2 no
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return false;
+  int is = known[dev].load();
+  if (!is) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(1024);
+    cfg.dynamicSmemBytes = kSortSmem;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 16;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    is = cudaFuncSetAttribute(sort_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                 cudaFuncSetAttribute(sort_kernel<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem) == cudaSuccess &&
+                 cudaOccupancyMaxActiveClusters(&n, sort_kernel<16>, &cfg) == cudaSuccess && n > 0
+             ? 1
+             : 2;
+    cudaGetLastError();
+    known[dev].store(is);
+  }
+  return is == 1;
 }
 
 }  // namespace tokens
@@ -342,15 +436,18 @@ extern "C" int dsmoe_sort_tokens(const int64_t* idx, long long P, int k, int n_e
   DSMOE_REQUIRE(idx && pos && src && offsets, DSMOE_ERR_ARG, "sort_tokens: null pointer");
   DSMOE_REQUIRE(((uintptr_t)idx & 7) == 0 && (((uintptr_t)pos | (uintptr_t)src | (uintptr_t)offsets) & 3) == 0, DSMOE_ERR_ALIGN,
                 "sort_tokens: misaligned pointer");
-  tokens::SortArgs a{idx, pos, src, offsets, (int)(P * k), n_experts, 0};
-  const int C = a.n > 4096 ? 8 : 1;
-  int nw = (a.n / C + 127) / 128;  // a warp for each 128 pairs
-  nw = nw < 4 ? 4 : nw > 32 ? 32 : nw;
-  a.run = (int)((((long long)a.n + (long long)C * nw - 1) / (C * nw) + 31) / 32 * 32);
-  const size_t smem = ((size_t)(nw + 2) * n_experts + 32) * sizeof(int);
+  tokens::SortArgs a{idx, pos, src, offsets, (int)(P * k), n_experts, 0, 0};
+  // 131072 pairs of 384 experts: 26.8 us with 8 CTAs, 16.9 with 16 (24576 pairs 8.1 and 6.3; 12282: 6.5 and 6.6)
+  const int C = a.n > 16384 && tokens::sixteen() ? 16 : a.n > 4096 ? 8 : 1;
+  const int cw = (a.n / C + 127) / 128;  // a warp for each 128 pairs
+  a.cw = cw < 1 ? 1 : cw > 32 ? 32 : cw;
+  a.run = (int)((((long long)a.n + (long long)C * a.cw - 1) / (C * a.cw) + 31) / 32 * 32);
+  const int ew = (n_experts + 31) / 32;  // a thread for each expert in the scan
+  const int nw = a.cw > ew ? a.cw : ew;
+  const size_t smem = ((size_t)(a.cw + 2) * n_experts + 32) * sizeof(int);
+  auto kern = C == 1 ? tokens::sort_kernel<1> : C == 8 ? tokens::sort_kernel<8> : tokens::sort_kernel<16>;
   if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(tokens::sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (34 * tokens::kMaxExperts + 32) * (int)sizeof(int)) != cudaSuccess)
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, tokens::kSortSmem) != cudaSuccess)
     return cuda_status("sort_tokens");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(C);
@@ -362,8 +459,8 @@ extern "C" int dsmoe_sort_tokens(const int64_t* idx, long long P, int k, int n_e
   at.val.clusterDim.x = C;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, tokens::sort_kernel, a);
+  cfg.numAttrs = C > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, kern, a);
   return cuda_status("sort_tokens");
 }
 
