@@ -90,7 +90,17 @@ def test_python_surface_takes_cuda_tensors_only():
                  lambda: dsmoe.int8_grouped_gemm(q, s, q[None], s[None], order.offsets),
                  lambda: dsmoe.sort_tokens(torch.zeros(2, 1, dtype=torch.int64), 2),
                  lambda: dsmoe.dispatch_tokens(x, order), lambda: dsmoe.combine_tokens(x, order)):
-        with pytest.raises(ValueError, match="CUDA"):
+        with pytest.raises(ValueError, match=r"CUDA tensors only, got \[2, .*\] on cpu"):
+            call()
+
+
+def test_native_half_refuses_other_objects():
+    import dsmoe
+    from dsmoe import _ops
+    for call in (lambda: dsmoe.swiglu_quant(3), lambda: dsmoe.int8_gemm(None, None, None, None),
+                 lambda: dsmoe.rms_norm_quant(torch.ones(2), [1.0]), lambda: dsmoe.sort_tokens(torch.zeros(2, 1), None),
+                 lambda: dsmoe.int8_grouped_gemm(1, 2, 3, 4, None), lambda: _ops.combine_tokens(1, 2)):
+        with pytest.raises(TypeError):
             call()
 
 
