@@ -31,8 +31,6 @@ namespace gemm_i8 {
 constexpr int NT = 320;       // 10 warps
 constexpr int CT = 256;       // epilogue threads
 constexpr int TM = 128;       // weight rows per tile (MMA M)
-constexpr int MAXTT = 256;    // accumulator columns of one tile
-constexpr int SPLIT_TT = 64;  // the same where K is split over a cluster
 constexpr int MAXRS = 12;     // ring stages
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxK = 131071;
@@ -45,8 +43,10 @@ struct Args {
   const float* b_s;    // [E][N]
   const int* offsets;  // [E + 1], or null: one group of all M rows
   void* out;           // [M][N]
-  int M, N, K, E, nkb, TT, BR, RS, NTN, S, out_f32;
+  int M, N, K, E, nkb, TT, BR, RS, NTN, out_f32;
+  unsigned tcols;      // tensor memory columns (one-tile kernel)
 };
+
 
 struct Tile {
   int e, n0, m0, cols;  // expert, first channel, first token row, tokens
@@ -101,6 +101,11 @@ __device__ __forceinline__ uint32_t peer_addr(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void peer_arrive(uint64_t* bar, uint32_t rank) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_addr(smem_u32(bar), rank)) : "memory");
+}
+__device__ __forceinline__ int4 peer_ld4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ int peer_ld(uint32_t addr) {
   int v;
@@ -197,10 +202,25 @@ __device__ __forceinline__ Tile locate_tile(const Args& a, const int* first, con
   return Tile{lo, at / mt * rows_w, first[lo] + m, max(min(per, rows - m), 0)};
 }
 
-__device__ __forceinline__ void store_out(const Args& a, long long t, int n, float v) {
+// Four neighbouring channels of token t from n (a multiple of 4) on.
+__device__ __forceinline__ void store_out4(const Args& a, long long t, int n, const float (&v)[4]) {
   const long long o = t * a.N + n;
-  if (a.out_f32) reinterpret_cast<float*>(a.out)[o] = v;
-  else reinterpret_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(v);
+  if (a.N % 4 == 0 && ((uintptr_t)a.out & 15) == 0) {
+    if (a.out_f32) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+      *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(a.out) + o) =
+          make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= a.N) return;
+    if (a.out_f32) reinterpret_cast<float*>(a.out)[o + i] = v[i];
+    else reinterpret_cast<__nv_bfloat16*>(a.out)[o + i] = __float2bfloat16_rn(v[i]);
+  }
 }
 
 // Accumulators of this warp's 32 channels and every other 32 tokens from 32 `half` on -> out. sc: the tokens'
@@ -252,57 +272,64 @@ __device__ __forceinline__ void fill_behind(const Args& a, const Groups& g, int 
   }
 }
 
-template <bool SPLIT>
-__global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ Args a) {
+// A position in a ring of n stages and the parity of its current use, without divisions in the loops.
+struct Ring {
+  int s = 0;
+  uint32_t par = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++s == n) {
+      s = 0;
+      par ^= 1u;
+    }
+  }
+};
+
+// Programmatic dependent launch: a kernel that follows another in its stream may be set up (barriers, tensor
+// memory) before that one has ended; no global memory is touched before the wait.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// One tile per cluster of S CTAs (S = 1: per CTA): 128 weight rows x up to 256 tokens, each CTA a share of the K
+// blocks. The partial sums change hands through the ring's memory once the products have read it.
+template <int S>
+__global__ void __launch_bounds__(NT) gemm_i8_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t gsm[];
   uint8_t* ring = gsm + ((1024 - (smem_u32(gsm) & 1023)) & 1023);
-  const int SB = TM * 128 + a.TT * 128;  // stage bytes
-  int* part = reinterpret_cast<int*>(ring + a.RS * SB);                       // SPLIT: [2][TT][TM]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(part + (SPLIT ? 2 * a.TT * TM : 0));
+  const int SB = (TM + a.TT) * 128;  // stage bytes
+  int* part = reinterpret_cast<int*>(ring);  // [tokens][TM]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + a.RS * SB);
   uint64_t* full = bars;             // [MAXRS] stage landed
   uint64_t* empty = full + MAXRS;    // [MAXRS] stage read by its MMAs
-  uint64_t* accf = empty + MAXRS;    // [2] accumulator complete
-  uint64_t* acce = accf + 2;         // [2] accumulator read (8 warps)
-  uint64_t* pfull = acce + 2;        // [2] SPLIT: every CTA's partial written
-  uint64_t* pempty = pfull + 2;      // [2] SPLIT: this CTA's partial read by every CTA
-  uint64_t* mdone = pempty + 2;      // [1] no MMA in flight
-  float* scales = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(mdone + 1) + 15) & ~(uintptr_t)15);  // [2][SPLIT_TT]
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(scales + 2 * SPLIT_TT);
+  uint64_t* accf = empty + MAXRS;    // [1] accumulator complete
+  float* scales = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(accf + 1) + 15) & ~(uintptr_t)15);  // [256]
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(scales + 256);
   volatile int* abortf = reinterpret_cast<volatile int*>(tslot + 1);
   int* wsum = reinterpret_cast<int*>(tslot + 2);  // [10]
   int* first = wsum + 10;            // [E + 1] first row of each group
   int* pre = first + a.E + 1;        // [E + 1] tiles before each group
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int S = SPLIT ? a.S : 1;
-  const int rank = SPLIT ? blockIdx.x % S : 0;
-  const int cid = blockIdx.x / S, ncl = gridDim.x / S;
+  const int rank = blockIdx.x % S, tile = blockIdx.x / S;
   const int kb0 = rank * a.nkb / S, kb1 = (rank + 1) * a.nkb / S;
-
   if (tid == 0) {
-    for (int s = 0; s < MAXRS; ++s) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
+    for (int s = 0; s < a.RS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&accf[s], 1);
-      mbar_init(&acce[s], 8);
-      mbar_init(&pfull[s], S);
-      mbar_init(&pempty[s], S);
-    }
-    mbar_init(mdone, 1);
+    mbar_init(accf, 1);
     *abortf = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(a.tcols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
   const Groups g = setup_groups(a, first, pre, wsum);
-  const int tiles = g.tiles;
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (SPLIT) cluster_sync();  // every CTA's barriers exist before the first remote arrival
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tslot;
   auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
@@ -313,139 +340,110 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_kernel(const __grid_constant__ 
     }
     return true;
   };
-  auto locate = [&](int tile) -> Tile { return locate_tile<16>(a, first, pre, tile, TM); };
-
+  // the grid covers the most tiles that M rows in E groups can have
+  const bool work = tile < g.tiles;
+  const Tile t = work ? locate_tile<16>(a, first, pre, tile, TM) : Tile{0, 0, 0, 0};
   if (warp == 0) {
     if (lane == 0) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
-      int it = 0;
-      bool ok = true;
-      for (int tile = cid; tile < tiles && ok; tile += ncl) {
-        const Tile t = locate(tile);
-        const int nb = max((t.cols + a.BR - 1) / a.BR, 1);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % a.RS;
-          if (it >= a.RS && !wait(&empty[s], ((it / a.RS) - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          uint8_t* st = ring + s * SB;
-          mbar_expect_tx(&full[s], (uint32_t)(TM * 128 + nb * a.BR * 128));
-          tma_2d(st, &a.tb, kb * 128, t.e * a.N + t.n0, &full[s]);
-          for (int b = 0; b < nb; ++b) tma_2d(st + TM * 128 + b * a.BR * 128, &a.ta, kb * 128, t.m0 + b * a.BR, &full[s]);
-        }
+      pdl_launch();
+      const int nb = (t.cols + a.BR - 1) / a.BR, yb = t.e * a.N + t.n0;
+      const uint32_t bytes = (uint32_t)(TM * 128 + nb * a.BR * 128);
+      Ring p;
+      int issued = 0;
+      for (int kb = kb0; kb < kb1 && work; ++kb, p.next(a.RS), ++issued) {
+        if (issued >= a.RS && !wait(&empty[p.s], p.par ^ 1u)) break;
+        uint8_t* st = ring + p.s * SB;
+        mbar_expect_tx(&full[p.s], bytes);
+        tma_2d(st, &a.tb, kb * 128, yb, &full[p.s]);
+        for (int b = 0; b < nb; ++b) tma_2d(st + TM * 128 + b * a.BR * 128, &a.ta, kb * 128, t.m0 + b * a.BR, &full[p.s]);
       }
       // every copy issued has landed before the CTA may exit (the last use of each stage)
-      for (int i = it - 1; i >= 0 && i >= it - a.RS; --i) mbar_wait(&full[i % a.RS], (i / a.RS) & 1, kWaitNs);
+      for (int i = issued - 1; i >= 0 && i >= issued - a.RS; --i) mbar_wait(&full[i % a.RS], (i / a.RS) & 1, kWaitNs);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && work) {
       // D s32, A and B s8, both K-major
-      const uint32_t idesc0 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TM >> 4) << 24);
+      const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TM >> 4) << 24) |
+                             ((uint32_t)(((t.cols + 15) >> 4) * 2) << 17);
       const uint64_t da0 = desc_sw128(smem_u32(ring)), db0 = desc_sw128(smem_u32(ring + TM * 128));
-      int it = 0, tc = 0;
-      bool ok = true;
-      for (int tile = cid; tile < tiles && ok; tile += ncl, ++tc) {
-        const Tile t = locate(tile);
-        const int ac = tc & 1;
-        if (tc >= 2 && !wait(&acce[ac], ((tc >> 1) - 1) & 1)) break;
+      Ring p;
+      for (int kb = kb0; kb < kb1; ++kb, p.next(a.RS)) {
+        if (!wait(&full[p.s], p.par)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t idesc = idesc0 | ((uint32_t)(max((t.cols + 15) >> 4, 1) * 2) << 17);
-        const uint32_t d = tmem + (uint32_t)(ac * MAXTT);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % a.RS;
-          if (!wait(&full[s], (it / a.RS) & 1)) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t o = (uint64_t)(s * (SB >> 4));
+        const uint64_t o = (uint64_t)(p.s * (SB >> 4));
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mma_i8(d, da0 + o + 2u * q, db0 + o + 2u * q, idesc, (kb > kb0 || q > 0) ? 1u : 0u);
-          commit(&empty[s]);
-        }
-        commit(&accf[ac]);
+        for (int q = 0; q < 4; ++q) mma_i8(tmem, da0 + o + 2u * q, db0 + o + 2u * q, idesc, (kb > kb0 || q > 0) ? 1u : 0u);
+        commit(&empty[p.s]);
       }
-      commit(mdone);  // no MMA may still run when the tensor memory is freed
-      mbar_wait(mdone, 0, kWaitNs);
+      commit(accf);  // also after an abort: no MMA may still run when the tensor memory is freed
+      mbar_wait(accf, 0, kWaitNs);
     }
   } else {
     const int ct = tid - 64;
     const int qd = warp & 3, half = (warp - 2) >> 2;
     const int row_l = 32 * qd + lane;
-    const float nanv = __int_as_float(0x7FC00000);
-    auto store = [&](long long t, int n, float v) { store_out(a, t, n, v); };
-    int tc = 0;
-    bool ok = true;
-    for (int tile = cid; tile < tiles; tile += ncl, ++tc) {
-      const Tile t = locate(tile);
-      const int ac = tc & 1;
-      const int n = t.n0 + row_l;
-      float bs = 0.f;
-      float* sc = scales + ac * SPLIT_TT;
-      if (!SPLIT) {
-        // the tile's scales, while its products are still running (the other half of the buffer is being read)
-        if (n < a.N) bs = a.b_s[(long long)t.e * a.N + n];
-        if (ct < SPLIT_TT) sc[ct] = ct < t.cols ? a.a_s[t.m0 + ct] : 0.f;
-        named_bar_sync(1, CT);
-      }
-      ok = ok && wait(&accf[ac], (tc >> 1) & 1);
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const int groups = (t.cols + 15) >> 4;  // 16 tokens at a time, the two warps of a quadrant in turn
-      const uint32_t tq = tmem + ((uint32_t)(32 * qd) << 16) + (uint32_t)(ac * MAXTT);
-      if (!SPLIT) {
-        drain(a, tq, half, t.cols, t.m0, n, bs, sc, ok);
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acce[ac]);
-      } else {
-        int* mine = part + ac * a.TT * TM;
-        if (ok && tc >= 2) {
-          ok = cluster_wait(&pempty[ac], ((tc >> 1) - 1) & 1, kWaitNs);
-          if (!ok) *abortf = 1;
-        }
-        for (int c16 = half; c16 < groups; c16 += 2) {
-          int v[16];
-          ld16(tq + 16u * c16, v);
+    // S > 1: this CTA finishes channels rank TM / S .. of the tile, a thread four of them for one token at a time
+    constexpr int kQuads = TM / S / 4;
+    const int r = rank * (TM / S) + ct % kQuads * 4, n = t.n0 + (S > 1 ? r : row_l);
+    float bs[S > 1 ? 4 : 1];
+    // the scales, while the products are still running
+    if (work) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) mine[(16 * c16 + i) * TM + row_l] = v[i];
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acce[ac]);
-        asm volatile("fence.acq_rel.cluster;" ::: "memory");
-        named_bar_sync(1, CT);
-        if (ct < S) peer_arrive(&pfull[ac], (uint32_t)ct);
-        if (ok) {
-          ok = cluster_wait(&pfull[ac], (tc >> 1) & 1, kWaitNs);
-          if (!ok) *abortf = 1;
-        }
-        // this CTA finishes channels rank TM / S .. of the tile, for every token
-        const int rows = TM / S, r = rank * rows + ct % rows, nr = t.n0 + r;
-        if (nr < a.N) {
-          bs = a.b_s[(long long)t.e * a.N + nr];
-          for (int c = ct / rows; c < t.cols; c += CT / rows) {
-            const uint32_t at = smem_u32(mine + c * TM + r);
-            int sum = 0;
-            if (ok)
-              for (int z = 0; z < S; ++z) sum += peer_ld(peer_addr(at, (uint32_t)z));
-            store(t.m0 + c, nr, ok ? (float)sum * a.a_s[t.m0 + c] * bs : nanv);
+      for (int i = 0; i < (S > 1 ? 4 : 1); ++i) bs[i] = n + i < a.N ? a.b_s[(long long)t.e * a.N + n + i] : 0.f;
+      scales[ct] = ct < t.cols ? a.a_s[t.m0 + ct] : 0.f;
+    }
+    bool ok = work && wait(accf, 0) && !*abortf;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tq = tmem + ((uint32_t)(32 * qd) << 16);
+    if (S == 1) {
+      named_bar_sync(1, CT);
+      if (work) drain(a, tq, half, t.cols, t.m0, n, bs[0], scales, ok);
+    } else if (work) {
+      for (int c16 = half; 16 * c16 < t.cols; c16 += 2) {
+        int v[16];
+        ld16(tq + 16u * c16, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (16 * c16 + i < t.cols) part[(16 * c16 + i) * TM + row_l] = v[i];
+      }
+    }
+    if (S > 1) {
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (work && n < a.N) {
+        for (int c = ct / kQuads; c < t.cols; c += CT / kQuads) {
+          const uint32_t at = smem_u32(part + c * TM + r);
+          int4 v[S];
+          int bad = 0;
+#pragma unroll
+          for (int z = 0; z < S; ++z) v[z] = peer_ld4(peer_addr(at, (uint32_t)z));
+#pragma unroll
+          for (int z = 0; z < S; ++z) bad |= peer_ld(peer_addr(smem_u32(const_cast<int*>(abortf)), (uint32_t)z));
+          int sum[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int z = 0; z < S; ++z) {
+            sum[0] += v[z].x;
+            sum[1] += v[z].y;
+            sum[2] += v[z].z;
+            sum[3] += v[z].w;
           }
+          float o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = bad ? __int_as_float(0x7FC00000) : (float)sum[i] * bs[i] * scales[c];
+          store_out4(a, t.m0 + c, n, o);
         }
-        named_bar_sync(1, CT);
-        if (ct < S) peer_arrive(&pempty[ac], (uint32_t)ct);
       }
     }
     fill_behind(a, g, ct);
   }
   __syncwarp();
+  if (S > 1 && warp < 2) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (SPLIT) cluster_sync();  // no CTA leaves while another may still read its partials
+  // no CTA leaves while another may still read its partials: those reads are done when their sums are
+  if (S > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   if (warp == 1) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tcols) : "memory");
   }
 }
 
@@ -498,6 +496,8 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = blockIdx.x & 1, cid = blockIdx.x >> 1, ncl = gridDim.x >> 1;
   if (tid == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
     for (int s = 0; s < PRS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -514,6 +514,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
+  pdl_wait();
   const Groups g = setup_groups(a, first, pre, wsum);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
@@ -538,8 +539,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
 
   if (warp == 0) {
     if (lane == 0) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
+      pdl_launch();
       int it = 0;
       bool ok = true;
       for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
@@ -670,9 +670,11 @@ int device_limits(const char* name, int* sms, int* optin) {
   if (*sms && dev < 64) return DSMOE_OK;
   if (cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
       cudaDeviceGetAttribute(optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess ||
-      cudaFuncSetAttribute(gemm_i8_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_i8_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_i8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess ||
-      cudaFuncSetAttribute(gemm_i8_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess)
+      cudaFuncSetAttribute(gemm_i8_kernel<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, *optin) != cudaSuccess)
     return cuda_status(name);
   known[slot][1].store(*optin, std::memory_order_release);
   known[slot][0].store(*sms, std::memory_order_release);
@@ -689,6 +691,39 @@ int encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* m, const void* p, 
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   DSMOE_REQUIRE(r == CUDA_SUCCESS, DSMOE_ERR_CUDA, "int8_gemm: cuTensorMapEncodeTiled failed (%d)", (int)r);
   return DSMOE_OK;
+}
+
+struct Plan {
+  bool pair;
+  int TT, S;  // tokens per tile; CTAs of a cluster
+};
+
+Plan plan(long long M, long long N, int nkb, int E, int sms) {
+  // tokens of a tile: the mean group's, in the next of 16, 32 or 64; beyond that CTA pairs
+  const long long mean = E ? (M + E - 1) / E : M;
+  Plan p{mean > 64, mean <= 16 ? 16 : mean <= 32 ? 32 : 64, 1};
+  if (p.pair) {
+    p.TT = PTT;
+    p.S = 2;
+    if (!E) {
+      // the tile width that costs least: rounds of the pairs times a tile's columns, with the time that a
+      // tile costs beside its MMAs (filling the ring, storing the last accumulators) as 64 columns
+      const long long ntn = (N + 2 * TM - 1) / (2 * TM);
+      long long best = 0;
+      for (long long mt = (M + PTT - 1) / PTT; mt <= (M + 63) / 64; ++mt) {
+        const long long per = ((M + mt - 1) / mt + 31) / 32 * 32;
+        const long long cost = (mt * ntn + sms / 2 - 1) / (sms / 2) * (per + 64);
+        if (!best || cost < best) {
+          best = cost;
+          p.TT = (int)per;
+        }
+      }
+    }
+    return p;
+  }
+  const long long tiles = (N + TM - 1) / TM * (E ? M / p.TT + std::min<long long>(E, M) : (M + p.TT - 1) / p.TT);
+  while (p.S < 8 && p.S * 2 <= nkb && tiles * p.S * 2 <= sms) p.S *= 2;
+  return p;
 }
 
 int run(const char* name, const int8_t* x, const float* a_s, long long M, long long K, const int8_t* b, const float* b_s,
@@ -715,61 +750,47 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   a.nkb = (int)((K + 127) / 128);
   a.NTN = (int)((N + TM - 1) / TM);
   a.out_f32 = out_dtype == DSMOE_DTYPE_F32;
-  // tokens of a tile: the mean group's, in the next of 16, 32 or 64; beyond that CTA pairs
-  const long long mean = offsets ? (M + E - 1) / E : M;
-  const long long groups = offsets ? std::min<long long>(E, M) : 1;
-  const bool pair = mean > SPLIT_TT;
-  a.TT = mean <= 16 ? 16 : mean <= 32 ? 32 : SPLIT_TT;
-  a.S = 1;
-  a.BR = a.TT;
-  if (pair) {
-    a.NTN = (int)((N + 2 * TM - 1) / (2 * TM));
-    a.TT = PTT;
-    a.S = 2;
-    a.BR = PBR;
-    if (!offsets) {
-      // the tile width that costs least: rounds of the pairs times a tile's columns, with the time that a
-      // tile costs beside its MMAs (filling the ring, storing the last accumulators) as 64 columns
-      long long best = 0;
-      for (long long mt = (M + PTT - 1) / PTT; mt <= (M + 63) / 64; ++mt) {
-        const long long per = ((M + mt - 1) / mt + 31) / 32 * 32;
-        const long long cost = (mt * a.NTN + sms / 2 - 1) / (sms / 2) * (per + 64);
-        if (!best || cost < best) {
-          best = cost;
-          a.TT = (int)per;
-        }
-      }
-    }
-  }
-  const long long tiles = a.NTN * (M / a.TT + groups);  // at most
-  DSMOE_REQUIRE(tiles < (1LL << 31), DSMOE_ERR_ARG, "%s: too many tiles", name);
-  if (!pair)
-    while (a.S < 8 && a.S * 2 <= a.nkb && tiles * a.S * 2 <= sms) a.S *= 2;
+  const Plan p = plan(M, N, a.nkb, offsets ? E : 0, sms);
+  a.TT = p.TT;
+  a.BR = p.pair ? PBR : offsets ? std::min(p.TT, 64) : p.TT;
+  a.NTN = (int)((N + (p.pair ? 2 : 1) * TM - 1) / ((p.pair ? 2 : 1) * TM));
+  const long long tiles = a.NTN * (M / a.TT + (offsets ? std::min<long long>(E, M) : M % a.TT != 0));  // at most
+  DSMOE_REQUIRE(tiles * p.S < (1LL << 31), DSMOE_ERR_ARG, "%s: too many tiles", name);
   rc = encode(fn, &a.tb, b, K, (long long)E * N, TM);
   if (!rc) rc = encode(fn, &a.ta, x, K, M, a.BR);
   if (rc) return rc;
-  const size_t tables = (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
-  size_t smem;
-  if (pair) {
-    smem = 1024 + PRS * PSB + tables;
-  } else {
+  const size_t tables = 1024 + (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
+  size_t smem = tables + PRS * PSB;
+  if (!p.pair) {
     const int SB = (TM + a.TT) * 128;
-    const size_t fixed = 1024 + (a.S > 1 ? 2 * a.TT * TM * 4 : 0) + tables;
-    a.RS = (int)std::min<size_t>(MAXRS, (optin - fixed) / SB);
-    smem = fixed + (size_t)a.RS * SB;
+    // a stage for each K block of the CTA, as far as half of an SM's shared memory goes, so that two CTAs share
+    // an SM (one is set up or finished while the other loads); at least what the partial sums take
+    int rs = (int)((115 * 1024 - tables) / SB);
+    const int need = (a.TT * TM * 4 + SB - 1) / SB, most = (int)((optin - tables) / SB);
+    rs = std::max(rs, std::max(need, 4));
+    rs = std::min(rs, std::min(most, std::max((a.nkb + p.S - 1) / p.S, need)));
+    a.RS = std::min(rs, MAXRS);
+    a.tcols = a.TT <= 32 ? 32 : a.TT <= 64 ? 64 : a.TT <= 128 ? 128 : 256;
+    smem = tables + (size_t)a.RS * SB;
   }
-  auto kern = pair ? gemm_i8_pair_kernel : a.S > 1 ? gemm_i8_kernel<true> : gemm_i8_kernel<false>;
+  auto kern = p.pair     ? gemm_i8_pair_kernel
+              : p.S == 1 ? gemm_i8_kernel<1>
+              : p.S == 2 ? gemm_i8_kernel<2>
+              : p.S == 4 ? gemm_i8_kernel<4>
+                         : gemm_i8_kernel<8>;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(std::min<long long>(tiles, std::max(1, sms / a.S)) * a.S));
+  cfg.gridDim = dim3((unsigned)((p.pair ? std::min<long long>(tiles, sms / 2) : tiles) * p.S));
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = a.S;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = a.S > 1 ? 1 : 0;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = p.S;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.S > 1 ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kern, a);
   return cuda_status(name);
 }
