@@ -410,15 +410,16 @@ __global__ void __launch_bounds__(NT) gemm_i8_kernel(const __grid_constant__ Arg
     if (S > 1) {
       asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
       if (work && n < a.N) {
+        int bad = 0;
+#pragma unroll
+        for (int z = 0; z < S; ++z) bad |= peer_ld(peer_addr(smem_u32(const_cast<int*>(abortf)), (uint32_t)z));
         for (int c = ct / kQuads; c < t.cols; c += CT / kQuads) {
           const uint32_t at = smem_u32(part + c * TM + r);
           int4 v[S];
-          int bad = 0;
-#pragma unroll
-          for (int z = 0; z < S; ++z) v[z] = peer_ld4(peer_addr(at, (uint32_t)z));
-#pragma unroll
-          for (int z = 0; z < S; ++z) bad |= peer_ld(peer_addr(smem_u32(const_cast<int*>(abortf)), (uint32_t)z));
           int sum[4] = {0, 0, 0, 0};
+          // every CTA begins with its neighbour's partial, so that no CTA's memory is read by all at once
+#pragma unroll
+          for (int z = 0; z < S; ++z) v[z] = peer_ld4(peer_addr(at, (uint32_t)((rank + 1 + z) % S)));
 #pragma unroll
           for (int z = 0; z < S; ++z) {
             sum[0] += v[z].x;
@@ -453,9 +454,9 @@ __global__ void __launch_bounds__(NT) gemm_i8_kernel(const __grid_constant__ Arg
 // 256, one for each half of the tile's tokens) reads both CTAs' shared memory and writes each CTA's 128 rows
 // of accumulators into that CTA's tensor memory.
 constexpr int PTT = 512;                   // tokens per tile
-constexpr int PSB = TM * 128 + PTT / 2 * 128;  // stage bytes of one CTA: 16 KB of weights, 32 KB of tokens
-constexpr int PRS = 4;                     // stages
 constexpr int PBR = 64;                    // token rows of one load
+// Token rows of one CTA in a stage: half of the tile's, in whole loads; halves of 256 tokens lie 128 rows apart.
+__host__ __device__ inline int pair_rows(int TT) { return TT > 256 ? 256 : (TT / 2 + PBR - 1) / PBR * PBR; }
 
 __device__ __forceinline__ void mma_i8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -480,10 +481,11 @@ __device__ __forceinline__ void tma_2d_pair(void* dst, const CUtensorMap* tm, in
 __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) uint8_t gsm[];
   uint8_t* ring = gsm + ((1024 - (smem_u32(gsm) & 1023)) & 1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + PRS * PSB);
-  uint64_t* full = bars;           // [PRS] leader: both CTAs' stage landed
-  uint64_t* empty = full + PRS;    // [PRS] stage read by its MMAs
-  uint64_t* accf = empty + PRS;    // [2] half of the tensor memory: accumulators complete
+  const int SB = (TM + pair_rows(a.TT)) * 128;  // stage bytes of this CTA: its weight rows, its half of the tokens
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + a.RS * SB);
+  uint64_t* full = bars;           // [MAXRS] leader: both CTAs' stage landed
+  uint64_t* empty = full + MAXRS;  // [MAXRS] stage read by its MMAs
+  uint64_t* accf = empty + MAXRS;  // [2] half of the tensor memory: accumulators complete
   uint64_t* acce = accf + 2;       // [2] leader: accumulators read by both CTAs (8 warps each)
   uint64_t* mdone = acce + 2;      // [1] no MMA in flight
   float* scales = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(mdone + 1) + 15) & ~(uintptr_t)15);  // [2][256]
@@ -498,7 +500,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
   if (tid == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&a.tb) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&a.ta) : "memory");
-    for (int s = 0; s < PRS; ++s) {
+    for (int s = 0; s < a.RS; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -540,35 +542,37 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
   if (warp == 0) {
     if (lane == 0) {
       pdl_launch();
-      int it = 0;
+      int issued = 0;
+      Ring p;
       bool ok = true;
       for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
         const Tile t = locate(tile);
         const int w0 = width(t.cols, 0), w1 = width(t.cols, 1);
         const int nb0 = (w0 / 2 + PBR - 1) / PBR, nb1 = (w1 / 2 + PBR - 1) / PBR;
-        const int y0 = t.m0 + rank * (w0 / 2), y1 = t.m0 + w0 + rank * (w1 / 2);
-        for (int kb = 0; kb < a.nkb; ++kb, ++it) {
-          const int s = it % PRS;
-          if (it >= PRS && !wait(&empty[s], ((it / PRS) - 1) & 1)) {
+        const int y0 = t.m0 + rank * (w0 / 2), y1 = t.m0 + w0 + rank * (w1 / 2), yb = t.e * a.N + t.n0 + rank * TM;
+        const uint32_t bytes = (uint32_t)(2 * (TM * 128 + (nb0 + nb1) * PBR * 128));
+        for (int kb = 0; kb < a.nkb; ++kb, p.next(a.RS), ++issued) {
+          if (issued >= a.RS && !wait(&empty[p.s], p.par ^ 1u)) {
             ok = false;
             break;
           }
-          uint8_t* st = ring + s * PSB;
-          if (rank == 0) mbar_expect_tx(&full[s], (uint32_t)(2 * (TM * 128 + (nb0 + nb1) * PBR * 128)));
-          const uint32_t bar = peer_addr(smem_u32(&full[s]), 0);
-          tma_2d_pair(st, &a.tb, kb * 128, t.e * a.N + t.n0 + rank * TM, bar);
+          uint8_t* st = ring + p.s * SB;
+          if (rank == 0) mbar_expect_tx(&full[p.s], bytes);
+          const uint32_t bar = peer_addr(smem_u32(&full[p.s]), 0);
+          tma_2d_pair(st, &a.tb, kb * 128, yb, bar);
           for (int b = 0; b < nb0; ++b) tma_2d_pair(st + TM * 128 + b * PBR * 128, &a.ta, kb * 128, y0 + b * PBR, bar);
           for (int b = 0; b < nb1; ++b) tma_2d_pair(st + TM * 128 + 16384 + b * PBR * 128, &a.ta, kb * 128, y1 + b * PBR, bar);
         }
       }
       // every copy issued has landed (its MMAs have read it) before the CTA may exit
-      for (int i = it - 1; i >= 0 && i >= it - PRS; --i) cluster_wait(&empty[i % PRS], (i / PRS) & 1, kWaitNs);
+      for (int i = issued - 1; i >= 0 && i >= issued - a.RS; --i) cluster_wait(&empty[i % a.RS], (i / a.RS) & 1, kWaitNs);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
       const uint32_t idesc0 = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(2 * TM >> 4) << 24);
       const uint64_t da0 = desc_sw128(smem_u32(ring)), db0 = desc_sw128(smem_u32(ring + TM * 128));
-      int it = 0, slot = 0;  // slots: halves of the tensor memory used so far
+      int slot = 0;  // halves of the tensor memory used so far
+      Ring p;
       bool ok = true;
       for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
         const Tile t = locate(tile);
@@ -579,14 +583,13 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t id0 = idesc0 | ((uint32_t)(w0 >> 3) << 17), id1 = idesc0 | ((uint32_t)(w1 >> 3) << 17);
         const uint32_t d0 = tmem + (uint32_t)((slot & 1) * 256), d1 = tmem + (uint32_t)(((slot + 1) & 1) * 256);
-        for (int kb = 0; kb < a.nkb; ++kb, ++it) {
-          const int s = it % PRS;
-          if (!wait(&full[s], (it / PRS) & 1)) {
+        for (int kb = 0; kb < a.nkb; ++kb, p.next(a.RS)) {
+          if (!wait(&full[p.s], p.par)) {
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint64_t o = (uint64_t)(s * (PSB >> 4));
+          const uint64_t o = (uint64_t)(p.s * (SB >> 4));
 #pragma unroll
           for (int q = 0; q < 4; ++q) mma_i8_pair(d0, da0 + o + 2u * q, db0 + o + 2u * q, id0, (kb > 0 || q > 0) ? 1u : 0u);
           if (w1) {
@@ -594,7 +597,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
             for (int q = 0; q < 4; ++q)
               mma_i8_pair(d1, da0 + o + 2u * q, db0 + o + 1024u + 2u * q, id1, (kb > 0 || q > 0) ? 1u : 0u);
           }
-          commit_pair(&empty[s]);
+          commit_pair(&empty[p.s]);
         }
         for (int h = 0; h < n; ++h) commit_pair(&accf[(slot + h) & 1]);
         slot += n;
@@ -698,32 +701,64 @@ struct Plan {
   int TT, S;  // tokens per tile; CTAs of a cluster
 };
 
-Plan plan(long long M, long long N, int nkb, int E, int sms) {
-  // tokens of a tile: the mean group's, in the next of 16, 32 or 64; beyond that CTA pairs
-  const long long mean = E ? (M + E - 1) / E : M;
-  Plan p{mean > 64, mean <= 16 ? 16 : mean <= 32 ? 32 : 64, 1};
-  if (p.pair) {
-    p.TT = PTT;
-    p.S = 2;
-    if (!E) {
-      // the tile width that costs least: rounds of the pairs times a tile's columns, with the time that a
-      // tile costs beside its MMAs (filling the ring, storing the last accumulators) as 64 columns
-      const long long ntn = (N + 2 * TM - 1) / (2 * TM);
-      long long best = 0;
-      for (long long mt = (M + PTT - 1) / PTT; mt <= (M + 63) / 64; ++mt) {
-        const long long per = ((M + mt - 1) / mt + 31) / 32 * 32;
-        const long long cost = (mt * ntn + sms / 2 - 1) / (sms / 2) * (per + 64);
-        if (!best || cost < best) {
-          best = cost;
-          p.TT = (int)per;
-        }
-      }
-    }
-    return p;
+// Stages of a one-tile CTA's ring: one for each of its K blocks, as far as half of an SM's shared memory goes (two
+// CTAs then share an SM, one set up or finished while the other loads), at least four, and what the partials take.
+int one_tile_stages(int TT, int kb, size_t tables, size_t optin) {
+  const size_t SB = (size_t)(TM + TT) * 128;
+  const int half = (int)((115 * 1024 - tables) / SB), need = (int)((TT * TM * 4 + SB - 1) / SB), most = (int)((optin - tables) / SB);
+  return std::min(std::min(std::max(half, std::max(need, 4)), std::max(kb, need)), std::min(most, MAXRS));
+}
+
+// The tile shape that should take least time, in us, by a model of what bounds each kernel, its constants fitted to
+// measurements on a B200 (M 1..4096, N 72..8192, K 64..8192). An SM takes in at most 105 bytes/ns, and no more than its
+// ring's bytes in a round trip (2.2 us for weights that come from memory, 1.4 where other tiles brought them to L2);
+// all weights come from memory at 6200 bytes/ns; a K block takes 0.25 us to issue and 0.34 in a pair.
+Plan plan(long long M, long long N, int nkb, int E, int sms, size_t tables, size_t optin) {
+  if (E) {
+    // Groups: sizes are known to the device alone. Few rows: every expert has few, one tile each, K shared by two or
+    // four CTAs while the tiles cannot fill the GPU (48 rows of 384 experts, N 512: S = 1 20.9 us, 2 19.2; 6 rows: 2
+    // 12.6, 4 9.3). Else pairs, which adapt a tile's width to its group (384 rows: 65.8 us, one-tile 64.2; 6144 rows:
+    // 165 and 172; 8000 rows of 8 experts 87 and 118): up to 128, 256 or 512 tokens by the mean group.
+    if (M > 64) return Plan{true, M < 32LL * E ? 128 : M < 256LL * E ? 256 : PTT, 2};
+    const long long tiles = (N + TM - 1) / TM * (M / 32 + std::min<long long>(E, M));
+    int S = 1;
+    while (S < 4 && S * 2 <= nkb && tiles * S * 2 <= 400) S *= 2;
+    return Plan{false, M <= 16 ? 16 : 32, S};
   }
-  const long long tiles = (N + TM - 1) / TM * (E ? M / p.TT + std::min<long long>(E, M) : (M + p.TT - 1) / p.TT);
-  while (p.S < 8 && p.S * 2 <= nkb && tiles * p.S * 2 <= sms) p.S *= 2;
-  return p;
+  Plan best{false, 16, 1};
+  double least = 1e30;
+  const double weights = (double)N * nkb * 128 / 6.2e6;
+  const long long ntn = (N + TM - 1) / TM;
+  const long long mt0 = (M + 255) / 256, mt1 = std::min<long long>((M + 15) / 16, mt0 + 15);
+  for (long long mt = mt0; mt <= mt1; ++mt) {
+    const int TT = (int)(((M + mt - 1) / mt + 15) / 16 * 16);
+    for (int S = 1; S <= 8 && S <= nkb; S *= 2) {
+      const int kb = (nkb + S - 1) / S, rs = one_tile_stages(TT, kb, tables, optin);
+      const double SB = (TM + TT) * 128.0;
+      const int occ = tables + rs * SB <= 113 * 1024 ? 2 : 1;
+      const int fit = S == 8 ? sms * 13 / 15 : S == 4 ? sms * 14 / 15 : sms;  // SMs that clusters of S can use
+      const long long n = (M + TT - 1) / TT * ntn * S, rounds = (n + fit - 1) / fit, waves = (rounds + occ - 1) / occ;
+      const double load = std::max(std::max(kb * SB * std::min<long long>(occ, rounds) / 105e3, kb * (1.4 + 0.8 / mt) / rs), 0.25 * kb);
+      // joining partials costs a cluster barrier and each CTA's share of the reads
+      const double t = 0.8 + std::max(waves * load, weights) + waves * (2.2 + (S > 1 ? 0.5 + 0.0125 * TT + 0.1 * S : 0.008 * TT));
+      if (t < least) least = t, best = Plan{false, TT, S};
+    }
+  }
+  if (M > 64) {
+    const long long ntp = (N + 2 * TM - 1) / (2 * TM);
+    const long long mp0 = (M + PTT - 1) / PTT, mp1 = std::min<long long>((M + 63) / 64, mp0 + 15);
+    for (long long mt = mp0; mt <= mp1; ++mt) {
+      const int TT = (int)(((M + mt - 1) / mt + 31) / 32 * 32);
+      const double SB = (TM + pair_rows(TT)) * 128.0;
+      const long long rounds = ((M + TT - 1) / TT * ntp + sms / 2 - 1) / (sms / 2);
+      // a K block: its MMAs, or its bytes; a tile of more than 256 tokens is stored before the next one begins
+      const double block = std::max(0.34, std::max(TT * 0.00105, SB / 105e3)), store = 0.012 * TT;
+      const double tile = TT > 256 ? nkb * block + store : std::max(nkb * block, 1.2 * store);
+      const double t = 5.0 + std::max(rounds * tile, weights) + (TT > 256 ? 0.0 : store);
+      if (t < least) least = t, best = Plan{true, TT, 2};
+    }
+  }
+  return best;
 }
 
 int run(const char* name, const int8_t* x, const float* a_s, long long M, long long K, const int8_t* b, const float* b_s,
@@ -750,7 +785,8 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   a.nkb = (int)((K + 127) / 128);
   a.NTN = (int)((N + TM - 1) / TM);
   a.out_f32 = out_dtype == DSMOE_DTYPE_F32;
-  const Plan p = plan(M, N, a.nkb, offsets ? E : 0, sms);
+  const size_t tables = 1024 + (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
+  const Plan p = plan(M, N, a.nkb, offsets ? E : 0, sms, tables, optin);
   a.TT = p.TT;
   a.BR = p.pair ? PBR : offsets ? std::min(p.TT, 64) : p.TT;
   a.NTN = (int)((N + (p.pair ? 2 : 1) * TM - 1) / ((p.pair ? 2 : 1) * TM));
@@ -759,20 +795,14 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   rc = encode(fn, &a.tb, b, K, (long long)E * N, TM);
   if (!rc) rc = encode(fn, &a.ta, x, K, M, a.BR);
   if (rc) return rc;
-  const size_t tables = 1024 + (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
-  size_t smem = tables + PRS * PSB;
-  if (!p.pair) {
-    const int SB = (TM + a.TT) * 128;
-    // a stage for each K block of the CTA, as far as half of an SM's shared memory goes, so that two CTAs share
-    // an SM (one is set up or finished while the other loads); at least what the partial sums take
-    int rs = (int)((115 * 1024 - tables) / SB);
-    const int need = (a.TT * TM * 4 + SB - 1) / SB, most = (int)((optin - tables) / SB);
-    rs = std::max(rs, std::max(need, 4));
-    rs = std::min(rs, std::min(most, std::max((a.nkb + p.S - 1) / p.S, need)));
-    a.RS = std::min(rs, MAXRS);
+  const int SB = (TM + (p.pair ? pair_rows(a.TT) : a.TT)) * 128;
+  if (p.pair) {
+    a.RS = std::min(MAXRS, (int)((optin - tables) / SB));
+  } else {
+    a.RS = one_tile_stages(a.TT, (a.nkb + p.S - 1) / p.S, tables, optin);
     a.tcols = a.TT <= 32 ? 32 : a.TT <= 64 ? 64 : a.TT <= 128 ? 128 : 256;
-    smem = tables + (size_t)a.RS * SB;
   }
+  const size_t smem = tables + (size_t)a.RS * SB;
   auto kern = p.pair     ? gemm_i8_pair_kernel
               : p.S == 1 ? gemm_i8_kernel<1>
               : p.S == 2 ? gemm_i8_kernel<2>
