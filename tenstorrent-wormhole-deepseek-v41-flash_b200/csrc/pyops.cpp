@@ -3,10 +3,14 @@
 // written in Python cost 10 to 17 us a call, here 4 to 6. The compute is libdsmoe.so's, through include/dsmoe.h.
 //
 // Errors: ValueError / TypeError for arguments (the messages name the operator), dsmoe.DsmoeError for a failing
-// entry point, torch's own exceptions (out of memory) as they are. No C++ exception leaves a function.
+// entry point, torch's own exceptions (out of memory) as they are. No C++ exception leaves a function. The gradients
+// of dispatch and combine are autograd functions of their own here: backward runs without Python.
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/tensor_dtypes.h>
 
 #include <ATen/cuda/EmptyTensor.h>
@@ -21,6 +25,8 @@
 #include <optional>
 #include <sstream>
 #include <string>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/dsmoe.h"
 
@@ -33,10 +39,12 @@ constexpr int64_t kMaxExperts = 1024, kMaxTopk = 64, kMaxRow = 16384, kMaxK = 13
 
 PyObject* g_error = nullptr;  // dsmoe._lib.DsmoeError
 
-// A refusal: caught at the entry points and raised in Python.
+// A refusal, caught at the entry points and raised in Python. type: nullptr with code DSMOE_OK where the Python
+// error is set already, nullptr with another code for a failing entry point.
 struct Refused {
-  PyObject* type;  // nullptr: the Python error is set already
+  PyObject* type;
   std::string what;
+  int code = DSMOE_OK;
 };
 
 template <typename... A>
@@ -104,14 +112,7 @@ void run(const Tensor& t, F call) {
   std::optional<c10::cuda::CUDAGuard> guard;
   if (c10::cuda::current_device() != i) guard.emplace(i);
   const int rc = call(static_cast<void*>(c10::cuda::getCurrentCUDAStream(i).stream()));
-  if (rc != DSMOE_OK) {
-    PyObject* e = PyObject_CallFunction(g_error ? g_error : PyExc_RuntimeError, "is", rc, dsmoe_last_error());
-    if (e) {
-      PyErr_SetObject(reinterpret_cast<PyObject*>(Py_TYPE(e)), e);
-      Py_DECREF(e);
-    }
-    throw Refused{nullptr, ""};
-  }
+  if (rc != DSMOE_OK) throw Refused{nullptr, dsmoe_last_error(), rc};
 }
 
 PyObject* wrap(const Tensor& t) {
@@ -136,7 +137,15 @@ PyObject* guarded(PyObject* const* args, Py_ssize_t n, Py_ssize_t expected, F f)
   try {
     return f(args);
   } catch (const Refused& r) {
-    if (r.type) PyErr_SetString(r.type, r.what.c_str());
+    if (r.type) {
+      PyErr_SetString(r.type, r.what.c_str());
+    } else if (r.code != DSMOE_OK) {
+      PyObject* e = PyObject_CallFunction(g_error ? g_error : PyExc_RuntimeError, "is", r.code, r.what.c_str());
+      if (e) {
+        PyErr_SetObject(reinterpret_cast<PyObject*>(Py_TYPE(e)), e);
+        Py_DECREF(e);
+      }
+    }
     return nullptr;
   }
   END_HANDLE_TH_ERRORS
@@ -313,31 +322,156 @@ void check_order(const char* name, const Tensor& pos, const Tensor& off) {
               name, "order must come from sort_tokens");
 }
 
+// xs, and the scales of xs where s is defined
+std::pair<Tensor, Tensor> dispatch(const char* name, const Tensor& x0, const Tensor& pos, const Tensor& off, Tensor s) {
+  same_device(name, {&x0, &pos, &off, &s});
+  check_order(name, pos, off);
+  const int64_t P = pos.size(0), k = pos.size(1);
+  value_check(x0.dim() == 2 && x0.size(0) == P && x0.size(1) > 0, name, "x must be [", P, ", width], got ", x0.sizes());
+  if (s.defined()) {
+    want(name, s, "scales", at::kFloat, {P});
+    no_grad(name, {&x0, &s});
+    s = dense(s, false);
+  }
+  const Tensor x = dense(x0, false);
+  Tensor xs = empty(x, {P * k, x.size(1)}, x.scalar_type()), ss = s.defined() ? empty(x, {P * k}, at::kFloat) : Tensor();
+  if (P)
+    run(x, [&](void* st) {
+      return dsmoe_dispatch_rows(ptr(x), static_cast<const float*>(ptr(s)), static_cast<const int*>(ptr(pos)),
+                                 static_cast<const int*>(ptr(off)), static_cast<int>(off.size(0) - 1), P, static_cast<int>(k),
+                                 x.size(1) * static_cast<int64_t>(x.element_size()), ptr(xs), static_cast<float*>(ptr(ss)), st);
+    });
+  return {xs, ss};
+}
+
+Tensor combine(const char* name, const Tensor& y0, const Tensor& pos, const Tensor& off, Tensor wt) {
+  same_device(name, {&y0, &pos, &off, &wt});
+  check_order(name, pos, off);
+  const int dt = float_code(name, y0, "ys");
+  const int64_t P = pos.size(0), k = pos.size(1);
+  value_check(y0.dim() == 2 && y0.size(0) == P * k && y0.size(1) > 0, name, "ys must be [", P * k, ", width], got ", y0.sizes());
+  if (wt.defined()) {
+    want(name, wt, "wt", at::kFloat, pos.sizes());
+    wt = dense(wt, false);
+  }
+  const Tensor ys = dense(y0, false);
+  Tensor y = empty(ys, {P, ys.size(1)}, ys.scalar_type());
+  if (P)
+    run(ys, [&](void* st) {
+      return dsmoe_combine_rows(ptr(ys), dt, static_cast<const int*>(ptr(pos)), static_cast<const float*>(ptr(wt)), P,
+                                static_cast<int>(k), ys.size(1), ptr(y), st);
+    });
+  return y;
+}
+
+// ------------------------------------------------------------------ gradients
+
+// A gradient captured into a CUDA graph must not reach a leaf whose accumulation node was made outside the capture
+// (a live eager graph holds it): autograd would run that node on the stream it was made on and break the capture.
+void check_capture(const char* name, std::initializer_list<const Tensor*> ts) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) todo.push_back(torch::autograd::impl::gradient_edge(*t).function);
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    const auto node = todo.back();
+    todo.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+      const auto stream = node->stream();
+      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+      bool inside = true;
+      if (stream) {
+        // an error is the legacy stream's answer while another stream is being captured
+        inside = cudaStreamIsCapturing(c10::cuda::CUDAStream(*stream).stream(), &status) == cudaSuccess &&
+                 status != cudaStreamCaptureStatusNone;
+        if (!inside) cudaGetLastError();
+      }
+      if (!inside)
+        refuse(PyExc_RuntimeError, name,
+               "a gradient cannot be captured while an eager graph of the same leaf is alive; delete its outputs first");
+    }
+    for (const auto& e : node->next_edges()) todo.push_back(e.function);
+  }
+}
+
+// f() on an autograd thread, where a refusal is a torch error; differentiable once
+template <typename F>
+auto in_backward(const char* name, std::initializer_list<const Tensor*> ts, F f) {
+  if (c10::GradMode::is_enabled())
+    for (const Tensor* t : ts)
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->requires_grad(), name, ": differentiable once (create_graph is not supported)");
+  try {
+    return f();
+  } catch (const Refused& r) {
+    TORCH_CHECK(false, name, ": ", r.what);
+  }
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& pos, const Tensor& off) {
+    ctx->save_for_backward({pos, off});
+    return dispatch("dispatch_tokens", x, pos, off, Tensor()).first;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const char* name = "dispatch_tokens (gradient)";
+    const Tensor dx = in_backward(name, {&g[0]}, [&] { return combine(name, g[0], saved[0], saved[1], Tensor()); });
+    return {dx, Tensor(), Tensor()};
+  }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& ys, const std::optional<Tensor>& weights,
+                        const Tensor& pos, const Tensor& off) {
+    const Tensor wt = weights ? *weights : Tensor();
+    // the rows are needed for the weights' gradient alone
+    ctx->save_for_backward({wt.defined() && wt.requires_grad() ? ys : Tensor(), wt, pos, off});
+    return combine("combine_tokens", ys, pos, off, wt);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const char* name = "combine_tokens (gradient)";
+    const Tensor &ys0 = saved[0], &wt0 = saved[1], &pos = saved[2], &off = saved[3];
+    const bool need_ys = ctx->needs_input_grad(0), need_wt = wt0.defined() && ctx->needs_input_grad(1);
+    Tensor dys, dwt;
+    in_backward(name, {&g[0], &ys0, &wt0}, [&] {
+      const Tensor dy = dense(g[0], false), ys = need_wt ? dense(ys0, false) : Tensor(), wt = wt0.defined() ? dense(wt0, false) : wt0;
+      const int64_t P = pos.size(0), k = pos.size(1), H = dy.size(1);
+      if (need_ys) dys = empty(dy, {P * k, H}, dy.scalar_type());
+      if (need_wt) dwt = empty(dy, {P, k}, at::kFloat);
+      if (P && (need_ys || need_wt))
+        run(dy, [&](void* st) {
+          return dsmoe_combine_grad(ptr(dy), ptr(ys), float_code(name, dy, "dy"), static_cast<const int*>(ptr(pos)),
+                                    static_cast<const float*>(ptr(wt)), static_cast<const int*>(ptr(off)),
+                                    static_cast<int>(off.size(0) - 1), P, static_cast<int>(k), H, ptr(dys),
+                                    static_cast<float*>(ptr(dwt)), st);
+        });
+      return 0;
+    });
+    return {dys, dwt, Tensor(), Tensor()};
+  }
+};
+
+bool wants_grad(const Tensor& t) { return c10::GradMode::is_enabled() && t.defined() && t.requires_grad(); }
+
 // x, pos, offsets, scales -> xs, or (xs, ss)
 PyObject* dispatch_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(args, n, 4, [](PyObject* const* args) -> PyObject* {
     const char* name = "dispatch_tokens";
-    const Tensor &x0 = tensor(name, args[0]), &pos = tensor(name, args[1]), &off = tensor(name, args[2]);
-    Tensor s = maybe(name, args[3]);
-    same_device(name, {&x0, &pos, &off, &s});
-    check_order(name, pos, off);
-    const int64_t P = pos.size(0), k = pos.size(1);
-    value_check(x0.dim() == 2 && x0.size(0) == P && x0.size(1) > 0, name, "x must be [", P, ", width], got ", x0.sizes());
+    const Tensor &x = tensor(name, args[0]), &pos = tensor(name, args[1]), &off = tensor(name, args[2]);
+    const Tensor s = maybe(name, args[3]);
     if (s.defined()) {
-      want(name, s, "scales", at::kFloat, {P});
-      no_grad(name, {&x0, &s});
-      s = dense(s, false);
+      const auto r = dispatch(name, x, pos, off, s);
+      return tuple({&r.first, &r.second});
     }
-    const Tensor x = dense(x0, false);
-    Tensor xs = empty(x, {P * k, x.size(1)}, x.scalar_type()), ss = s.defined() ? empty(x, {P * k}, at::kFloat) : Tensor();
-    if (P)
-      run(x, [&](void* st) {
-        return dsmoe_dispatch_rows(ptr(x), static_cast<const float*>(ptr(s)), static_cast<const int*>(ptr(pos)),
-                                   static_cast<const int*>(ptr(off)), static_cast<int>(off.size(0) - 1), P, static_cast<int>(k),
-                                   x.size(1) * static_cast<int64_t>(x.element_size()), ptr(xs), static_cast<float*>(ptr(ss)), st);
-      });
-    if (s.defined()) return tuple({&xs, &ss});
-    return wrap(xs);
+    if (!wants_grad(x)) return wrap(dispatch(name, x, pos, off, s).first);
+    type_check(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat, name,
+               "a gradient needs bfloat16 or float32, got ", x.scalar_type());
+    same_device(name, {&x, &pos, &off});
+    check_capture(name, {&x});
+    return wrap(Dispatch::apply(x, pos, off));
   });
 }
 
@@ -345,46 +479,12 @@ PyObject* dispatch_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* combine_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded(args, n, 4, [](PyObject* const* args) -> PyObject* {
     const char* name = "combine_tokens";
-    const Tensor &y0 = tensor(name, args[0]), &pos = tensor(name, args[1]), &off = tensor(name, args[2]);
-    Tensor wt = maybe(name, args[3]);
-    same_device(name, {&y0, &pos, &off, &wt});
-    check_order(name, pos, off);
-    const int dt = float_code(name, y0, "ys");
-    const int64_t P = pos.size(0), k = pos.size(1);
-    value_check(y0.dim() == 2 && y0.size(0) == P * k && y0.size(1) > 0, name, "ys must be [", P * k, ", width], got ", y0.sizes());
-    if (wt.defined()) {
-      want(name, wt, "wt", at::kFloat, pos.sizes());
-      wt = dense(wt, false);
-    }
-    const Tensor ys = dense(y0, false);
-    Tensor y = empty(ys, {P, ys.size(1)}, ys.scalar_type());
-    if (P)
-      run(ys, [&](void* st) {
-        return dsmoe_combine_rows(ptr(ys), dt, static_cast<const int*>(ptr(pos)), static_cast<const float*>(ptr(wt)), P,
-                                  static_cast<int>(k), ys.size(1), ptr(y), st);
-      });
-    return wrap(y);
-  });
-}
-
-// dy, ys (None without dwt), pos, offsets, wt, whether dys, whether dwt -> (dys, dwt); of combine_tokens' own tensors
-PyObject* combine_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  return guarded(args, n, 7, [](PyObject* const* args) -> PyObject* {
-    const char* name = "combine_tokens (gradient)";
-    const Tensor &d0 = tensor(name, args[0]), &pos = tensor(name, args[2]), &off = tensor(name, args[3]);
-    const Tensor y0 = maybe(name, args[1]), w0 = maybe(name, args[4]);
-    const Tensor dy = dense(d0, false), ys = y0.defined() ? dense(y0, false) : y0, wt = w0.defined() ? dense(w0, false) : w0;
-    const int64_t P = pos.size(0), k = pos.size(1), H = dy.size(1);
-    Tensor dys = args[5] == Py_True ? empty(dy, {P * k, H}, dy.scalar_type()) : Tensor();
-    Tensor dwt = args[6] == Py_True ? empty(dy, {P, k}, at::kFloat) : Tensor();
-    if (P && (dys.defined() || dwt.defined()))
-      run(dy, [&](void* st) {
-        return dsmoe_combine_grad(ptr(dy), ptr(ys), float_code(name, dy, "dy"), static_cast<const int*>(ptr(pos)),
-                                  static_cast<const float*>(ptr(wt)), static_cast<const int*>(ptr(off)),
-                                  static_cast<int>(off.size(0) - 1), P, static_cast<int>(k), H, ptr(dys),
-                                  static_cast<float*>(ptr(dwt)), st);
-      });
-    return tuple({&dys, &dwt});
+    const Tensor &ys = tensor(name, args[0]), &pos = tensor(name, args[1]), &off = tensor(name, args[2]);
+    const Tensor wt = maybe(name, args[3]);
+    if (!wants_grad(ys) && !wants_grad(wt)) return wrap(combine(name, ys, pos, off, wt));
+    same_device(name, {&ys, &pos, &off, &wt});
+    check_capture(name, {&ys, &wt});
+    return wrap(Combine::apply(ys, wt.defined() ? std::optional<Tensor>(wt) : std::nullopt, pos, off));
   });
 }
 
@@ -402,7 +502,6 @@ PyMethodDef kMethods[] = {{"rms_norm_quant", DSMOE_FAST(rms_norm_quant)},
                           {"sort_tokens", DSMOE_FAST(sort_tokens)},
                           {"dispatch_tokens", DSMOE_FAST(dispatch_tokens)},
                           {"combine_tokens", DSMOE_FAST(combine_tokens)},
-                          {"combine_grad", DSMOE_FAST(combine_grad)},
                           {"set_error_type", set_error_type, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", "Native half of dsmoe.ops.", -1, kMethods};

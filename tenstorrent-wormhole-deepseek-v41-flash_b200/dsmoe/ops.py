@@ -93,61 +93,12 @@ def sort_tokens(idx: torch.Tensor, n_experts: int) -> TokenOrder:
     return TokenOrder._make(_ops.sort_tokens(idx, n_experts))
 
 
-def _eager_leaf(name: str, *ts):
-    """A gradient captured into a CUDA graph must not reach a leaf whose accumulation node belongs to a
-    live eager graph: autograd runs that node on the stream it was made on, outside the capture. The
-    node carries a mark from the eager call, so that the captured call can refuse. Returns the nodes,
-    which live only as long as something holds them: hold them until the call's own graph does."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    nodes = []
-    for t in ts:
-        if t is not None and t.requires_grad and t.is_leaf:
-            node = torch.autograd.graph.get_gradient_edge(t).node
-            nodes.append(node)
-            if not capturing:
-                node.metadata["dsmoe_eager"] = True
-            elif node.metadata.get("dsmoe_eager"):
-                raise RuntimeError(f"{name}: an eager graph of this leaf is still alive; delete its outputs before "
-                                   "capturing a backward pass")
-    return nodes
-
-
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, pos, offsets):
-        ctx.save_for_backward(pos, offsets)
-        return _ops.dispatch_tokens(x, pos, offsets, None)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dxs):
-        return _ops.combine_tokens(dxs, *ctx.saved_tensors, None), None, None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ys, pos, offsets, wt):
-        ctx.save_for_backward(ys if ctx.needs_input_grad[3] else None, pos, offsets, wt)
-        return _ops.combine_tokens(ys, pos, offsets, wt)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        need = ctx.needs_input_grad
-        dys, dwt = _ops.combine_grad(dy, *ctx.saved_tensors, need[0], need[3])
-        return dys, None, None, dwt
-
-
 def dispatch_tokens(x: torch.Tensor, order: TokenOrder, scales: Optional[torch.Tensor] = None):
     """xs [tokens * k, width]: row order.pos[t, j] is x[t]; rows behind the last are zero.
 
     x [tokens, width] of any dtype. With ``scales`` [tokens] fp32 (8-bit rows) returns (xs, scales of xs).
-    The gradient of x (bf16 or fp32) is the sum of its rows' gradients, in fp32, in order of j."""
-    if scales is None and torch.is_grad_enabled() and x.requires_grad:
-        if x.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"dispatch_tokens: a gradient needs bfloat16 or float32, got {x.dtype}")
-        nodes = _eager_leaf("dispatch_tokens", x)  # noqa: F841  (held over the call)
-        return _Dispatch.apply(x, order.pos, order.offsets)
+    The gradient of x (bf16 or fp32) is the sum of its rows' gradients, in fp32, in order of j. It can be captured
+    into a CUDA graph; a capture beside a live eager graph of the same leaves is refused. Differentiable once."""
     return _ops.dispatch_tokens(x, order.pos, order.offsets, scales)
 
 
@@ -155,8 +106,5 @@ def combine_tokens(ys: torch.Tensor, order: TokenOrder, wt: Optional[torch.Tenso
     """y [tokens, width] = sum over j of wt[t, j] * ys[order.pos[t, j]]: summed in fp32 in order of j, rounded
     once to ys's dtype (bf16 or fp32). Dropped choices add nothing. wt [tokens, k] fp32, None: ones.
 
-    Differentiable in ys (rows behind the last get zero) and wt."""
-    if torch.is_grad_enabled() and (ys.requires_grad or (wt is not None and wt.requires_grad)):
-        nodes = _eager_leaf("combine_tokens", ys, wt)  # noqa: F841  (held over the call)
-        return _Combine.apply(ys, order.pos, order.offsets, wt)
+    Differentiable (once) in ys (rows behind the last get zero) and wt; captures as in ``dispatch_tokens``."""
     return _ops.combine_tokens(ys, order.pos, order.offsets, wt)

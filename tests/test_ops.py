@@ -558,20 +558,34 @@ def test_backward_in_a_graph(ops):
 
 
 def test_backward_capture_refused_beside_a_live_eager_graph(ops):
-    """The refusal's own logic, without a capture that would go wrong: the mark on the leaf's node."""
-    from dsmoe import ops as O
+    """The captured call is refused before it launches anything; without the eager graph it runs."""
     order = ops.sort_tokens(choices(96, 4, 2, 3), 3)
-    x = rnd(97, 4, 16).requires_grad_()
-    xs = ops.dispatch_tokens(x, order)
-    real = torch.cuda.is_current_stream_capturing
-    try:
-        torch.cuda.is_current_stream_capturing = lambda: True
+    x, wt, d = rnd(97, 4, 16).requires_grad_(), rnd(98, 4, 2).requires_grad_(), rnd(99, 4, 16)
+    f = lambda: ops.combine_tokens(ops.dispatch_tokens(x * 2.0, order), order, wt)  # x reaches it through another node
+    alive = f()
+    want = torch.autograd.grad(f(), (x, wt), d)
+    for _ in range(2):
         with pytest.raises(RuntimeError, match="eager graph"):
-            ops.dispatch_tokens(x, order)
-        del xs
-        O._eager_leaf("dispatch_tokens", x)  # the eager graph is gone
-    finally:
-        torch.cuda.is_current_stream_capturing = real
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                f()
+    torch.cuda.synchronize()
+    del alive
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(f(), (x, wt), d)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_differentiable_once(ops):
+    order = ops.sort_tokens(choices(110, 4, 2, 3), 3)
+    x, wt = rnd(111, 4, 16).requires_grad_(), rnd(112, 4, 2).requires_grad_()
+    y = ops.combine_tokens(ops.dispatch_tokens(x, order), order, wt)
+    with pytest.raises(NotImplementedError, match="once"):
+        torch.autograd.grad(y.sum(), (x, wt), create_graph=True)
+    with torch.no_grad():
+        assert not ops.combine_tokens(ops.dispatch_tokens(x, order), order, wt).requires_grad
 
 
 def test_int8_experts_layer(ops):

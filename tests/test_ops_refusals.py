@@ -83,13 +83,14 @@ def test_token_entry_points_refuse():
 def test_python_surface_takes_cuda_tensors_only():
     import dsmoe
     x, w = torch.zeros(2, 128), torch.ones(128)
-    q, s = torch.zeros(2, 128, dtype=torch.int8), torch.ones(2)
+    q, s, g = torch.zeros(2, 128, dtype=torch.int8), torch.ones(2), torch.zeros(2, 128, requires_grad=True)
     order = dsmoe.TokenOrder(torch.zeros(2, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32),
                              torch.zeros(3, dtype=torch.int32))
     for call in (lambda: dsmoe.rms_norm_quant(x, w), lambda: dsmoe.swiglu_quant(x), lambda: dsmoe.int8_gemm(q, s, q, s),
                  lambda: dsmoe.int8_grouped_gemm(q, s, q[None], s[None], order.offsets),
                  lambda: dsmoe.sort_tokens(torch.zeros(2, 1, dtype=torch.int64), 2),
-                 lambda: dsmoe.dispatch_tokens(x, order), lambda: dsmoe.combine_tokens(x, order)):
+                 lambda: dsmoe.dispatch_tokens(x, order), lambda: dsmoe.combine_tokens(x, order),
+                 lambda: dsmoe.dispatch_tokens(g, order), lambda: dsmoe.combine_tokens(g, order)):
         with pytest.raises(ValueError, match=r"CUDA tensors only, got \[2, .*\] on cpu"):
             call()
 
