@@ -135,14 +135,16 @@ DSMOE_API int dsmoe_act_quant(const void* x, int x_dtype, long long M, long long
  * multiple of 128, pow2 as there, s [rows, hidden / 128]), DSMOE_DTYPE_I8 with one scale per row,
  * s = max(amax, 1e-4) / 127, q = rint(v / s), s [rows]. residual_out (r; may be residual or x itself)
  * and normed (v rounded to dtype) may be NULL. dtype F32 or BF16, weight [hidden] F32 or BF16, hidden
- * <= 16384. A row (E4M3: a block) with an infinity or NaN gets the scale NaN. E4M3 wants 16-byte
- * aligned pointers. Feeds dsmoe_fp8_gemm / dsmoe_int8_gemm. */
+ * <= 16384. Squares are summed in fp32; a row with an infinity or NaN, or whose squares overflow, gets NaN
+ * scales. Pointers other than s are 16-byte aligned; q, s, residual_out and normed overlap nothing else.
+ * Feeds dsmoe_fp8_gemm / dsmoe_int8_gemm. */
 DSMOE_API int dsmoe_rms_norm_quant(const void* x, int dtype, const void* residual, const void* weight, int w_dtype,
                                    long long rows, long long hidden, float eps, int q_dtype, int pow2, void* q, float* s,
                                    void* residual_out, void* normed, void* stream);
 
 /* v = silu(min(g, limit)) * clamp(u, -limit, limit) * row_weight[row] (NULL: 1) for gu [rows, 2 inter] =
- * g | u, quantized as above: the expert FFN's activation (dsv41/tt/moe.py:133-139) between two 8-bit
+ * g | u, quantized as above (NaN scales for a row, E4M3: a block, whose amax is not finite; gu and q 16-byte
+ * aligned): the expert FFN's activation (dsv41/tt/moe.py:133-139) between two 8-bit
  * products. */
 DSMOE_API int dsmoe_swiglu_quant(const void* gu, int dtype, const float* row_weight, long long rows, long long inter,
                                  float limit, int q_dtype, int pow2, void* q, float* s, void* stream);

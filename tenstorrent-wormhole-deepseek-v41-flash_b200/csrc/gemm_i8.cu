@@ -802,7 +802,13 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
     a.RS = one_tile_stages(a.TT, (a.nkb + p.S - 1) / p.S, tables, optin);
     a.tcols = a.TT <= 32 ? 32 : a.TT <= 64 ? 64 : a.TT <= 128 ? 128 : 256;
   }
-  const size_t smem = tables + (size_t)a.RS * SB;
+  // Shared memory also decides who shares an SM, and with it its tensor memory, whose allocation waits without a limit
+  // while CTAs of a cluster wait for one another. A pair (all 512 columns) takes the whole SM; a CTA of a cluster half of
+  // it: two such CTAs hold at most 512 columns, and no kernel that takes more than half an SM, as those with pairs of
+  // their own do, can stand between the CTAs of one cluster.
+  size_t smem = tables + (size_t)a.RS * SB;
+  if (p.pair) smem = optin;
+  else if (p.S > 1) smem = std::max<size_t>(smem, 113 * 1024);
   auto kern = p.pair     ? gemm_i8_pair_kernel
               : p.S == 1 ? gemm_i8_kernel<1>
               : p.S == 2 ? gemm_i8_kernel<2>

@@ -10,7 +10,8 @@
 // stays in registers between. The norm needs two values of the whole row, sum(r^2) and (int8)
 // max|r w|: since amax(v) = max|r w| / sqrt(..), both come out of one block reduction, so a row costs
 // one barrier. r is the rounded residual (what the next layer adds to), sums and products are fp32.
-// A row (e4m3: a block) whose amax is not finite gets the scale NaN, so its values read back as NaN.
+// Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
+// or NaN or whose squares overflow fp32, and of a swiglu's row (e4m3: block) whose amax is not finite.
 #include "common.cuh"
 
 namespace dsmoe {
@@ -217,8 +218,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 __device__ __forceinline__ float scale_of(float amax, float inv_top, int pow2) {
-  float s = (amax < kAmaxFloor ? kAmaxFloor : amax) * inv_top;  // a NaN stays
+  amax = amax < kAmaxFloor ? kAmaxFloor : amax;  // a NaN stays
+  float s = amax * inv_top;
   if (pow2) {
+    s = amax / 448.0f;  // exact where it is a power of 2: the product with the reciprocal may lie above
     int e;
     const float m = frexpf(s, &e);
     if (s < INFINITY) s = ldexpf(1.0f, m == 0.5f ? e - 1 : e);
@@ -316,6 +319,11 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
   }
 }
 
+// NaN where the squares' sum is not finite: a row with an infinity or NaN, or with values past 1e19.
+__device__ __forceinline__ float rstd_of(float sum, const Args& a) {
+  return sum < INFINITY ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : __int_as_float(0x7FC00000);
+}
+
 // One row in registers: residual added and stored, squares and |r w| reduced; v holds r w afterwards.
 template <typename T, int NV, bool FP8, bool EDGE>
 __device__ __forceinline__ void norm_row(const Args& a, const Raw<T> (&x)[NV], const Raw<T> (&r)[NV],
@@ -393,7 +401,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
   float v[NV][VEC], sum, top;
   norm_row<T, NV, FP8, EDGE>(a, x, r, v, sum, top, row, t, live);
   row_reduce<true, !FP8>(sum, top, a.tpr, 0);
-  const float rstd = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+  const float rstd = rstd_of(sum, a);
   store_normed<T, NV, EDGE>(a, v, rstd, row, t, live);
   quant_store<VEC, NV, FP8, EDGE>(a, v, rstd, top, row, t, live);
 }
@@ -445,7 +453,7 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
     row_reduce<true, !FP8>(sum, top, a.tpr, i & 1);  // its barrier: every thread has read the stage
     if (t == 0 && row + kStages * step < a.rows) fetch(row + kStages * step, s);
     // an expired wait leaves a row of NaN
-    const float rstd = ok ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : __int_as_float(0x7FC00000);
+    const float rstd = ok ? rstd_of(sum, a) : __int_as_float(0x7FC00000);
     store_normed<T, NV, false>(a, v, rstd, row, t, true);
     quant_store<VEC, NV, FP8, false>(a, v, rstd, top, row, t, true);
   }

@@ -49,7 +49,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional[tor
     ``int8_gemm``. ``normed``: also v in x's dtype (the router's input). ``inplace``: the new residual is
     written over ``residual``, which must be contiguous.
 
-    v is quantized from fp32. A row (fp8: a block of 128) holding an infinity or NaN has the scale NaN."""
+    v is quantized from fp32. A row holding an infinity or NaN, or whose squares overflow fp32, has NaN scales."""
     return NormQuant._make(_ops.rms_norm_quant(x, weight, residual, eps, fmt, scale_fmt is not None, bool(normed),
                                                bool(inplace)))
 
@@ -59,8 +59,8 @@ def swiglu_quant(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, *,
     """(q, s) of silu(min(g, limit)) * clamp(u, -limit, limit) * row_weight for gu [..., 2 * inter] = g | u.
 
     The activation of ``Expert`` (dsv41/tt/moe.py:133-139) between two 8-bit products; formats and scales
-    as in ``rms_norm_quant``. ``row_weight`` [...] fp32 (e.g. routing weights) is applied before the
-    quantization."""
+    as in ``rms_norm_quant``; a row (fp8: a block) whose amax is not finite has the scale NaN. ``row_weight``
+    [...] fp32 (e.g. routing weights) is applied before the quantization."""
     return _ops.swiglu_quant(gu, row_weight, limit, fmt, scale_fmt is not None)
 
 

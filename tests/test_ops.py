@@ -137,12 +137,18 @@ def test_rms_norm_quant_special_rows(ops, fmt):
     _, v = norm_ref(x, w, None)
     check_quant(got.q[ok], got.s[ok], v[ok], fmt, 32 * U)
     assert not got.q[1].float().any() and bool(torch.isfinite(got.s[1]).all())
-    assert bool(torch.isnan(vals[2]).all())  # a NaN spoils its row's mean
-    if fmt == "fp8":  # an infinity: its block; the mean is infinite, so the rest is zero
-        assert bool(torch.isnan(got.s[3, 1])) and not vals[3, 0].any()
-        assert bool(torch.isnan(got.s[4, 0])) and not vals[4, 1].any()
-    else:
-        assert bool(torch.isnan(vals[3:5]).all())
+    assert bool(torch.isnan(vals[2:5]).all()) and bool(torch.isnan(got.s[2:5]).all())
+    x[0, 7] = 3e30  # its square overflows: not a row of zeros
+    big = ops.rms_norm_quant(x[:1], w, fmt=fmt, normed=True)
+    assert bool(torch.isnan(big.s).all()) and bool(torch.isnan(big.normed).all())
+
+
+def test_power_of_two_scales_at_their_borders(ops):
+    x = torch.ones((1, 384), device="cuda")  # mean 1, eps 0: v is the weight, exactly
+    w = torch.full((384,), 0.25, device="cuda")
+    w[5], w[130], w[260] = 448.0, -3.5, 448.0 * (1 + 2.0 ** -23)
+    got = ops.rms_norm_quant(x, w, eps=0.0, scale_fmt="ue8m0")
+    assert got.s.tolist() == [[1.0, 2.0 ** -7, 2.0]]
 
 
 def swiglu_ref(gu, wr=None, limit=10.0):
@@ -163,6 +169,16 @@ def test_swiglu_quant(ops, fmt, rows, n, dtype):
     check_quant(q, s, swiglu_ref(gu), fmt, 16 * U)
     q, s = ops.swiglu_quant(gu, wr, limit=3.0, fmt=fmt)
     check_quant(q, s, swiglu_ref(gu, wr, 3.0), fmt, 17 * U)
+
+
+@pytest.mark.parametrize("fmt,rows,n", [("fp8", 12283, 2048), ("int8", 6001, 4096), ("int8", 24001, 136), ("int8", 9001, 1000),
+                                        ("fp8", 20000, 256)])
+def test_swiglu_quant_many_rows(ops, fmt, rows, n):
+    gu, wr = rnd(113, rows, 2 * n, dtype=torch.bfloat16, scale=4.0), rnd(114, rows)
+    gu[rows - 1, 3] = float("nan")
+    q, s = ops.swiglu_quant(gu, wr, fmt=fmt)
+    check_quant(q[:-1], s[:-1], swiglu_ref(gu, wr)[:-1], fmt, 17 * U)
+    assert bool(torch.isnan(s[-1]).any())
 
 
 def test_swiglu_quant_special_values(ops):
