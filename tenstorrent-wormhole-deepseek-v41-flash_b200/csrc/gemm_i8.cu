@@ -696,23 +696,25 @@ int encode(PFN_cuTensorMapEncodeTiled_v12000 fn, CUtensorMap* m, const void* p, 
   return DSMOE_OK;
 }
 
+constexpr size_t kHalfSmem = 113 * 1024;  // of a CTA that shares its SM: with 1 KB each for the system, 228 KB
+
 struct Plan {
   bool pair;
   int TT, S;  // tokens per tile; CTAs of a cluster
 };
 
-// Stages of a one-tile CTA's ring: one for each of its K blocks, as far as half of an SM's shared memory goes (two
-// CTAs then share an SM, one set up or finished while the other loads), at least four, and what the partials take.
+// Stages of a one-tile CTA's ring: four, which is 64 KB of weights in flight (8 x 4096 x 5120 with four 6.2 us, three
+// 6.2, five 6.3, six 7.2: more bytes in flight wait in memory's queues), or what the partials take; no more than K blocks.
 int one_tile_stages(int TT, int kb, size_t tables, size_t optin) {
   const size_t SB = (size_t)(TM + TT) * 128;
-  const int half = (int)((115 * 1024 - tables) / SB), need = (int)((TT * TM * 4 + SB - 1) / SB), most = (int)((optin - tables) / SB);
-  return std::min(std::min(std::max(half, std::max(need, 4)), std::max(kb, need)), std::min(most, MAXRS));
+  const int need = (int)((TT * TM * 4 + SB - 1) / SB);
+  return std::min(std::max(std::min(kb, 4), need), (int)((optin - tables) / SB));
 }
 
 // The tile shape that should take least time, in us, by a model of what bounds each kernel, its constants fitted to
 // measurements on a B200 (M 1..4096, N 72..8192, K 64..8192). An SM takes in at most 105 bytes/ns, and no more than its
 // ring's bytes in a round trip (2.2 us for weights that come from memory, 1.4 where other tiles brought them to L2);
-// all weights come from memory at 6200 bytes/ns; a K block takes 0.25 us to issue and 0.34 in a pair.
+// all weights come from memory at 6200 bytes/ns; a K block takes 0.33 us, 0.34 in a pair.
 Plan plan(long long M, long long N, int nkb, int E, int sms, size_t tables, size_t optin) {
   if (E) {
     // Groups: sizes are known to the device alone. Few rows: every expert has few, one tile each, K shared by two or
@@ -735,12 +737,12 @@ Plan plan(long long M, long long N, int nkb, int E, int sms, size_t tables, size
     for (int S = 1; S <= 8 && S <= nkb; S *= 2) {
       const int kb = (nkb + S - 1) / S, rs = one_tile_stages(TT, kb, tables, optin);
       const double SB = (TM + TT) * 128.0;
-      const int occ = tables + rs * SB <= 113 * 1024 ? 2 : 1;
+      const int occ = tables + rs * SB <= kHalfSmem ? 2 : 1;
       const int fit = S == 8 ? sms * 13 / 15 : S == 4 ? sms * 14 / 15 : sms;  // SMs that clusters of S can use
       const long long n = (M + TT - 1) / TT * ntn * S, rounds = (n + fit - 1) / fit, waves = (rounds + occ - 1) / occ;
-      const double load = std::max(std::max(kb * SB * std::min<long long>(occ, rounds) / 105e3, kb * (1.4 + 0.8 / mt) / rs), 0.25 * kb);
+      const double load = std::max(std::max(kb * SB * std::min<long long>(occ, rounds) / 105e3, ((double)kb / rs - 1) * (1.4 + 0.8 / mt)), 0.33 * kb);
       // joining partials costs a cluster barrier and each CTA's share of the reads
-      const double t = 0.8 + std::max(waves * load, weights) + waves * (2.2 + (S > 1 ? 0.5 + 0.0125 * TT + 0.1 * S : 0.008 * TT));
+      const double t = 0.8 + std::max(waves * load, weights) + waves * (2.2 + (S > 1 ? 0.4 + 0.0125 * TT + 0.1 * S : 0.008 * TT));
       if (t < least) least = t, best = Plan{false, TT, S};
     }
   }
@@ -808,7 +810,7 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   // their own do, can stand between the CTAs of one cluster.
   size_t smem = tables + (size_t)a.RS * SB;
   if (p.pair) smem = optin;
-  else if (p.S > 1) smem = std::max<size_t>(smem, 113 * 1024);
+  else if (p.S > 1) smem = std::max(smem, kHalfSmem);
   auto kern = p.pair     ? gemm_i8_pair_kernel
               : p.S == 1 ? gemm_i8_kernel<1>
               : p.S == 2 ? gemm_i8_kernel<2>
