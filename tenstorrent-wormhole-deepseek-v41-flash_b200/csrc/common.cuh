@@ -287,6 +287,10 @@ __device__ __forceinline__ double ld_cg_f64(const double* p) {
   asm volatile("ld.global.cg.f64 %0, [%1];" : "=d"(r) : "l"(p));
   return r;
 }
+// Programmatic dependent launch: a kernel that follows another in its stream may be set up (barriers, tensor
+// memory) before that one has ended; no global memory is touched before the wait.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void named_bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -297,6 +301,22 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
 namespace dsmoe {
 void set_error(const char* fmt, ...);
 int cuda_status(const char* where);  // DSMOE_OK or DSMOE_ERR_CUDA after a launch
+
+// A launch with programmatic dependent launch allowed: the kernel begins with pdl_wait.
+template <typename... P, typename... A>
+void launch_pdl(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
 }  // namespace dsmoe
 
 #define DSMOE_REQUIRE(cond, code, ...)          \

@@ -284,11 +284,6 @@ struct Ring {
   }
 };
 
-// Programmatic dependent launch: a kernel that follows another in its stream may be set up (barriers, tensor
-// memory) before that one has ended; no global memory is touched before the wait.
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // One tile per cluster of S CTAs (S = 1: per CTA): 128 weight rows x up to 256 tokens, each CTA a share of the K
 // blocks. The partial sums change hands through the ring's memory once the products have read it.
 template <int S>

@@ -378,6 +378,8 @@ __device__ __forceinline__ void store_normed(const Args& a, const float (&v)[NV]
 template <typename T, int NV, bool FP8, bool EDGE>
 __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(T);
+  pdl_wait();
+  pdl_launch();
   const int t = threadIdx.x;
   const long long row = (long long)blockIdx.x * a.rpc + threadIdx.y, total = a.rows * a.n;
   const bool live = row < a.rows;
@@ -422,6 +424,8 @@ __global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
     fence_mbar_init();
   }
   __syncthreads();
+  pdl_wait();
+  pdl_launch();
   auto fetch = [&](long long row, int s) {
     uint8_t* st = sm + (size_t)s * terms * row_bytes;
     mbar_expect_tx(&full[s], terms * row_bytes);
@@ -479,6 +483,8 @@ __device__ __forceinline__ float swiglu(float g, float u, float limit) {
 template <typename T, int NV, bool FP8, bool EDGE>
 __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(T);
+  pdl_wait();
+  pdl_launch();
   const int t = threadIdx.x;
   const long long row = (long long)blockIdx.x * a.rpc + threadIdx.y, total = 2 * a.rows * a.n;
   const bool live = row < a.rows;
@@ -534,8 +540,7 @@ int sm_count() {
 template <bool NORM, typename T, int NV, bool FP8, bool EDGE>
 void launch(const Args& a, cudaStream_t st) {
   const long long grid = (a.rows + a.rpc - 1) / a.rpc;
-  if (NORM) norm_kernel<T, NV, FP8, EDGE><<<(unsigned)grid, dim3(a.tpr, a.rpc), 0, st>>>(a);
-  else swiglu_kernel<T, NV, FP8, EDGE><<<(unsigned)grid, dim3(a.tpr, a.rpc), 0, st>>>(a);
+  launch_pdl(NORM ? norm_kernel<T, NV, FP8, EDGE> : swiglu_kernel<T, NV, FP8, EDGE>, dim3((unsigned)grid), dim3(a.tpr, a.rpc), 0, st, a);
 }
 template <bool NORM, typename T, bool FP8, bool EDGE>
 void launch_nv(const Args& a, int nv, cudaStream_t st) {
@@ -549,7 +554,7 @@ template <typename T, int NV, bool FP8>
 void launch_stream(const Args& a, int ctas, size_t smem, cudaStream_t st) {
   auto k = norm_stream_kernel<T, NV, FP8>;
   if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  k<<<ctas, a.tpr, smem, st>>>(a);
+  launch_pdl(k, dim3(ctas), dim3(a.tpr), smem, st, a);
 }
 
 template <bool NORM, typename T>

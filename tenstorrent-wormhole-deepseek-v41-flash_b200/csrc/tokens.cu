@@ -39,6 +39,8 @@ constexpr int kSortSmem = (34 * kMaxExperts + 32) * (int)sizeof(int);  // at mos
 
 template <int C>
 __global__ void __launch_bounds__(1024) sort_kernel(const SortArgs a) {
+  pdl_wait();
+  pdl_launch();
   extern __shared__ int sm[];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = C > 1 ? (int)cluster.block_rank() : 0;
@@ -154,6 +156,8 @@ template <typename U>
 __global__ void dispatch_kernel(const U* __restrict__ x, const float* __restrict__ s, const int* __restrict__ pos,
                                 const int* __restrict__ offsets, int E, int k, int n, long long units, U* __restrict__ xs,
                                 float* __restrict__ ss) {
+  pdl_wait();
+  pdl_launch();
   const long long t = blockIdx.x;
   __shared__ int place[kMaxTopk];
   if (threadIdx.x < k) {
@@ -228,6 +232,8 @@ constexpr int kRows = 4;
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256, 7) combine_kernel(const T* __restrict__ ys, const int* __restrict__ pos, const float* __restrict__ wt, int k, int n,
                                long long width, T* __restrict__ y) {
+  pdl_wait();
+  pdl_launch();
   const long long t = blockIdx.x;
   __shared__ int place[kMaxTopk];
   __shared__ float weight[kMaxTopk];
@@ -269,6 +275,8 @@ __global__ void __launch_bounds__(256, 6) combine_grad_kernel(const T* __restric
                                                               const int* __restrict__ pos, const float* __restrict__ wt,
                                                               const int* __restrict__ offsets, int E, int k, int n,
                                                               long long width, T* __restrict__ dys, float* __restrict__ dwt) {
+  pdl_wait();
+  pdl_launch();
   const int batches = (k + kRows - 1) / kRows;
   const long long t = blockIdx.x / batches;
   const int j0 = blockIdx.x % batches * kRows;
@@ -367,7 +375,8 @@ void dispatch(const void* x, const float* s, const int* pos, const int* offsets,
   const long long units = row_bytes / (long long)sizeof(U);
   int th = threads_for(units);
   if (th < k) th = 64;  // the first k threads read the places
-  dispatch_kernel<U><<<row_grid(P, units, th), th, 0, st>>>((const U*)x, s, pos, offsets, E, k, (int)(P * k), units, (U*)xs, ss);
+  launch_pdl(dispatch_kernel<U>, row_grid(P, units, th), dim3(th), 0, st, (const U*)x, s, pos, offsets, E, k, (int)(P * k), units,
+             (U*)xs, ss);
 }
 
 template <typename T>
@@ -378,8 +387,8 @@ void combine(const void* ys, const int* pos, const float* wt, long long P, int k
   int th = threads_for(units);
   if (th < k) th = 64;
   const dim3 grid = row_grid(P, units, th);
-  if (wide) combine_kernel<T, V><<<grid, th, 0, st>>>((const T*)ys, pos, wt, k, (int)(P * k), width, (T*)y);
-  else combine_kernel<T, 1><<<grid, th, 0, st>>>((const T*)ys, pos, wt, k, (int)(P * k), width, (T*)y);
+  launch_pdl(wide ? combine_kernel<T, V> : combine_kernel<T, 1>, grid, dim3(th), 0, st, (const T*)ys, pos, wt, k, (int)(P * k),
+             width, (T*)y);
 }
 
 template <typename T>
@@ -389,10 +398,8 @@ void combine_grad(const void* dy, const void* ys, const int* pos, const float* w
   int th = threads_for(wide ? width / V : width);
   if (th < 32 * kRows) th = 32 * kRows;  // a warp joins each choice's sums
   const int n = (int)(P * k), grid = (int)(P * ((k + kRows - 1) / kRows));
-  if (wide)
-    combine_grad_kernel<T, V><<<grid, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, n, width, (T*)dys, dwt);
-  else
-    combine_grad_kernel<T, 1><<<grid, th, 0, st>>>((const T*)dy, (const T*)ys, pos, wt, offsets, E, k, n, width, (T*)dys, dwt);
+  launch_pdl(wide ? combine_grad_kernel<T, V> : combine_grad_kernel<T, 1>, dim3(grid), dim3(th), 0, st, (const T*)dy, (const T*)ys,
+             pos, wt, offsets, E, k, n, width, (T*)dys, dwt);
 }
 
 // Whether the current device runs clusters of 16 CTAs (more than 8 is not portable); asked once per device.
@@ -454,12 +461,14 @@ extern "C" int dsmoe_sort_tokens(const int64_t* idx, long long P, int k, int n_e
   cfg.blockDim = dim3(nw * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = C;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = C > 1 ? 1 : 0;
+  cudaLaunchAttribute at[2]{};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = C;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = C > 1 ? 2 : 1;
   cudaLaunchKernelEx(&cfg, kern, a);
   return cuda_status("sort_tokens");
 }
