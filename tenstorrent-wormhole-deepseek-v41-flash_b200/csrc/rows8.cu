@@ -19,8 +19,6 @@ namespace rows8 {
 
 constexpr float kAmaxFloor = 1e-4f;
 constexpr int kMaxHidden = 16384;
-constexpr int kStages = 3;              // rows in a persistent CTA's ring
-constexpr int kMaxSmem = 227 * 1024;
 
 struct Args {
   const void* x;      // norm: [rows][n]; swiglu: [rows][2n] (g | u)
@@ -241,17 +239,15 @@ __device__ __forceinline__ uint32_t int8x4(float a, float b, float c, float d) {
 // One block reduction per row: sum and maximum (not negative) over the row's tpr threads. Numbers that are not
 // negative order like their bits, with infinity and NaN on top, so the maximum is an integer one.
 template <bool SUM, bool MAX>
-__device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr, int turn) {
+__device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     if (SUM) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   if (MAX) top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7FFFFFFFu));
   if (tpr == 32) return;  // a row is one warp
-  __shared__ float ssums[2][32];  // a second reduction (turn 1) may begin while the first is being read
-  __shared__ uint32_t smaxs[2][32];
-  float* ssum = ssums[turn];
-  uint32_t* smax = smaxs[turn];
+  __shared__ float ssum[32];
+  __shared__ uint32_t smax[32];
   const int lane = threadIdx.x & 31, nw = tpr >> 5, w0 = threadIdx.y * nw, warp = w0 + (threadIdx.x >> 5);
   if (lane == 0) {
     if (SUM) ssum[warp] = sum;
@@ -402,82 +398,78 @@ __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
   }
   float v[NV][VEC], sum, top;
   norm_row<T, NV, FP8, EDGE>(a, x, r, v, sum, top, row, t, live);
-  row_reduce<true, !FP8>(sum, top, a.tpr, 0);
+  row_reduce<true, !FP8>(sum, top, a.tpr);
   const float rstd = rstd_of(sum, a);
   store_normed<T, NV, EDGE>(a, v, rstd, row, t, live);
   quant_store<VEC, NV, FP8, EDGE>(a, v, rstd, top, row, t, live);
 }
 
-// Many rows: a persistent CTA walks rows blockIdx.x + i gridDim.x while bulk copies bring the next ones into a
-// ring of shared memory, so loads stay in flight over the reductions and stores of the rows before.
-constexpr uint64_t kWaitNs = 1000000000ull;
-
-template <typename T, int NV, bool FP8>
-__global__ void __launch_bounds__(512) norm_stream_kernel(const Args a) {
-  constexpr int VEC = 16 / sizeof(T);
-  extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ uint64_t full[kStages];
-  const int t = threadIdx.x, terms = a.res ? 2 : 1;
-  const uint32_t row_bytes = (uint32_t)(a.n * sizeof(T));
-  if (t == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
-    fence_mbar_init();
-  }
-  __syncthreads();
-  pdl_wait();
-  pdl_launch();
-  auto fetch = [&](long long row, int s) {
-    uint8_t* st = sm + (size_t)s * terms * row_bytes;
-    mbar_expect_tx(&full[s], terms * row_bytes);
-    bulk_g2s(st, reinterpret_cast<const T*>(a.x) + row * a.n, row_bytes, &full[s]);
-    if (a.res) bulk_g2s(st + row_bytes, reinterpret_cast<const T*>(a.res) + row * a.n, row_bytes, &full[s]);
-  };
-  const long long step = gridDim.x;
-  if (t == 0)
-    for (int s = 0; s < kStages; ++s)
-      if (blockIdx.x + s * step < a.rows) fetch(blockIdx.x + s * step, s);
-  int i = 0;
-  for (long long row = blockIdx.x; row < a.rows; row += step, ++i) {
-    const int s = i % kStages;
-    const bool ok = mbar_wait(&full[s], (i / kStages) & 1, kWaitNs);
-    const T* st = reinterpret_cast<const T*>(sm + (size_t)s * terms * row_bytes);
-    Raw<T> x[NV], r[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = j * a.tpr + t;
-      x[j].zero();
-      r[j].zero();
-      if (c * VEC < a.n) {
-        x[j].load(st + c * VEC);
-        if (a.res) r[j].load(st + a.n + c * VEC);
-      }
-    }
-    float v[NV][VEC], sum, top;
-    norm_row<T, NV, FP8, false>(a, x, r, v, sum, top, row, t, true);
-    row_reduce<true, !FP8>(sum, top, a.tpr, i & 1);  // its barrier: every thread has read the stage
-    if (t == 0 && row + kStages * step < a.rows) fetch(row + kStages * step, s);
-    // an expired wait leaves a row of NaN
-    const float rstd = ok ? rstd_of(sum, a) : __int_as_float(0x7FC00000);
-    store_normed<T, NV, false>(a, v, rstd, row, t, true);
-    quant_store<VEC, NV, FP8, false>(a, v, rstd, top, row, t, true);
-  }
+__device__ __forceinline__ float exp2_hw(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_hw(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Two fp32 values in a register pair: one instruction for both on this architecture.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_get(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
 }
 
-// silu(g) u with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + r) with t = -g log2(e) rounded and r = -g - t ln 2,
-// what the rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all that is
-// approximated; the argument's own rounding would cost |g| units. exp's argument stops at 87, where silu(g) is
-// below 1e-35, so that the reciprocal stays a normal number.
-__device__ __forceinline__ float swiglu(float g, float u, float limit) {
-  g = min_nan(g, limit);
-  u = max_nan(min_nan(u, limit), -limit);
+// silu(g) u of two values, with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + r) with t = -g log2(e) rounded and
+// r = -g - t ln 2, what the rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all
+// that is approximated; the argument's own rounding would cost |g| units. exp's argument stops at 87, where silu(g) is
+// below 1e-35, so that the reciprocal stays a normal number. PACKED: both values in one instruction where it exists
+// (12282 rows of 2048: e4m3 24.2 us, 25.3 one by one; int8 rows without an edge are faster one by one, 26.0 and 27.7).
+template <bool PACKED>
+__device__ __forceinline__ void swiglu2(float& g0, float& g1, float u0, float u1, float limit) {
+  g0 = min_nan(g0, limit);
+  g1 = min_nan(g1, limit);
+  u0 = max_nan(min_nan(u0, limit), -limit);
+  u1 = max_nan(min_nan(u1, limit), -limit);
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
-  const float a = max_nan(g, -87.0f);
-  const float t = a * -kLog2e, d = fmaf(t, -kLn2, -a);
-  float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  e = 1.0f + fmaf(e, d, e);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e));
-  return g * r * u;
+  const float a0 = min_nan(-g0, 87.0f), a1 = min_nan(-g1, 87.0f);
+  float t0, t1, e0, e1;
+  if constexpr (PACKED) {
+    const F2 a = f2(a0, a1), t = f2_mul(a, f2(kLog2e, kLog2e)), r = f2_fma(t, f2(-kLn2, -kLn2), a);
+    f2_get(t, t0, t1);
+    e0 = exp2_hw(t0);
+    e1 = exp2_hw(t1);
+    const F2 e = f2(e0, e1);
+    f2_get(f2_add(f2_fma(e, r, e), f2(1.0f, 1.0f)), t0, t1);
+    f2_get(f2_mul(f2_mul(f2(g0, g1), f2(rcp_hw(t0), rcp_hw(t1))), f2(u0, u1)), g0, g1);
+  } else {
+    t0 = a0 * kLog2e;
+    t1 = a1 * kLog2e;
+    e0 = exp2_hw(t0);
+    e1 = exp2_hw(t1);
+    g0 = g0 * rcp_hw(1.0f + fmaf(e0, fmaf(t0, -kLn2, a0), e0)) * u0;
+    g1 = g1 * rcp_hw(1.0f + fmaf(e1, fmaf(t1, -kLn2, a1), e1)) * u1;
+  }
 }
 
 template <typename T, int NV, bool FP8, bool EDGE>
@@ -516,7 +508,7 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
     x[j].get(v[j]);
     y[j].get(u);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[j][i] = swiglu(v[j][i], u[i], a.limit);
+    for (int i = 0; i < VEC; i += 2) swiglu2<FP8 || EDGE>(v[j][i], v[j][i + 1], u[i], u[i + 1], a.limit);
     if (EDGE && (p.lo != 0 || p.hi != VEC)) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
@@ -526,7 +518,7 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
     for (int i = 0; i < VEC; ++i)
       if (!FP8) top = max_nan(top, fabsf(v[j][i]));
   }
-  if (!FP8) row_reduce<false, true>(none, top, a.tpr, 0);
+  if (!FP8) row_reduce<false, true>(none, top, a.tpr);
   quant_store<VEC, NV, FP8, EDGE>(a, v, wr, top, row, t, live);
 }
 
@@ -550,47 +542,17 @@ void launch_nv(const Args& a, int nv, cudaStream_t st) {
   else if constexpr (EDGE && sizeof(T) == 4) launch<NORM, T, 8, FP8, EDGE>(a, st);  // the longest: 4097 chunks
 }
 
-template <typename T, int NV, bool FP8>
-void launch_stream(const Args& a, int ctas, size_t smem, cudaStream_t st) {
-  auto k = norm_stream_kernel<T, NV, FP8>;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  launch_pdl(k, dim3(ctas), dim3(a.tpr), smem, st, a);
-}
-
 template <bool NORM, typename T>
 int run(Args& a, bool fp8, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   const bool edge = a.n % V != 0;
   const int nchunk = edge ? (a.n - 2) / V + 2 : a.n / V;  // a row's chunks, at most
-  if (NORM && !edge) {
-    // ring of whole rows where every CTA of the persistent grid gets several of them
-    const int nv = nchunk <= 1024 ? 2 : 4;
-    const int tpr = ((nchunk + nv - 1) / nv + 31) / 32 * 32;
-    const size_t smem = (size_t)kStages * (a.res ? 2 : 1) * a.n * sizeof(T);
-    const int per_sm = (int)(kMaxSmem / (smem + 2048));  // beside static arrays and what the system keeps
-    const int sms = sm_count(), fit = per_sm < 2048 / tpr ? per_sm : 2048 / tpr;
-    if (tpr >= 128 && tpr <= 512 && fit >= 1 && a.rows >= 2LL * sms * fit) {
-      a.tpr = tpr;
-      a.rpc = 1;
-      const int ctas = sms * fit;
-      if (fp8) {
-        if (nv == 2) launch_stream<T, 2, true>(a, ctas, smem, st);
-        else launch_stream<T, 4, true>(a, ctas, smem, st);
-      } else {
-        if (nv == 2) launch_stream<T, 2, false>(a, ctas, smem, st);
-        else launch_stream<T, 4, false>(a, ctas, smem, st);
-      }
-      return cuda_status("rms_norm_quant");
-    }
-  }
-  // Chunks per thread: one while there are few rows (a row's loads at once over many threads: 300 rows of 2048
-  // int8 codes 2.6 us, 2.9 with four), up to four where the grid fills the GPU and a thread's fixed instructions
-  // count (12282 rows 26.8 us, 33.2 with one). A row keeps its 32 threads. With an edge one chunk is as fast as
-  // two (6000 rows of 2049 24.9 us, 26.8).
+  // Chunks per thread: one, so that a row's loads go out at once from many threads. The norm's fixed work per thread
+  // is worth two where the grid fills the GPU several times (4096 rows of 5120 32.7 us, 34.7 with one); with an edge
+  // one is as fast, and the swiglu loses (12282 rows of 2048 24.2 us, 27.6 with two). A row keeps 32 threads.
   int nv = 1;
   while ((nchunk + nv - 1) / nv > 1024) nv *= 2;
-  if (!edge && a.rows * nchunk >= 8192LL * sm_count())
-    while (nv < 4 && nchunk >= 64 * nv) nv *= 2;
+  if (NORM && !edge && nv == 1 && nchunk >= 64 && a.rows * nchunk >= 8192LL * sm_count()) nv = 2;
   a.tpr = ((nchunk + nv - 1) / nv + 31) / 32 * 32;
   a.rpc = a.tpr >= 256 ? 1 : 256 / a.tpr;
   if (a.rpc > a.rows) a.rpc = (int)a.rows;
