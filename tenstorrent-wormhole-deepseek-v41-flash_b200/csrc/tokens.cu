@@ -6,6 +6,9 @@
 // The order is that of (expert, token, choice): a stable counting sort, so nothing depends on the
 // order in which threads arrive. Choices outside 0..E-1 are dropped (pos = -1) and the rows behind
 // offsets[E] hold zeros.
+// The three row kernels are bound by memory: a token's row is read once for all its choices. Measured, bf16 rows of
+// 5120, 4096 tokens x 6: dispatch 49 us (6.0 TB/s), combine 48 us (6.1), its gradient 91 us (6.0). The sort is a chain
+// of latencies: 48 pairs 3.0 us, 12282 6.5, 131072 16.9.
 #include <cooperative_groups.h>
 
 #include <atomic>
