@@ -96,7 +96,7 @@ struct Raw<float> {
 };
 
 // Chunk at element e (a multiple of VEC) of an array of `total` elements; outside it: zeros. inner: the chunk is
-// known to lie inside (only a tensor's first and last row reach over its ends).
+// known to lie inside (only rows with less than a chunk behind them reach over the array's end).
 template <typename T>
 __device__ __forceinline__ Raw<T> load_inside(const T* p, long long e, long long total, bool inner) {
   constexpr int VEC = 16 / sizeof(T);
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const Args a) {
     r[j].zero();
     if (p.hi) {
       if constexpr (EDGE) {
-        const bool inner = row + 1 < a.rows;
+        const bool inner = (a.rows - 1 - row) * a.n >= VEC;
         x[j] = load_inside(reinterpret_cast<const T*>(a.x), p.e, total, inner);
         if (a.res) r[j] = load_inside(reinterpret_cast<const T*>(a.res), p.e, total, inner);
       } else {
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
     y[j].zero();
     if (p.hi) {
       if constexpr (EDGE) {  // the codes' chunks are aligned; g and u lie at their own offsets to them
-        const bool inner = row > 0 && row + 1 < a.rows;
+        const bool inner = (a.rows - 1 - row) * a.n >= VEC;  // 2 VEC values: a span is two chunks
         x[j] = load_any(gu, e, total, inner);
         y[j] = load_any(gu, e + a.n, total, inner);
       } else {

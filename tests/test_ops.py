@@ -97,6 +97,22 @@ def test_rms_norm_quant_many_rows(ops, fmt, rows, n):
     check_quant(one.q, one.s, norm_ref(x[last], w, None)[1], fmt, 32 * U)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 2, 34, 255])
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 7, 9])
+def test_rows_shorter_than_a_chunk(ops, rows, n, dtype):
+    """Rows of a few values: many in one 16-byte chunk, the last ones less than a chunk before the end."""
+    x, r, w = rnd(115, rows, n, dtype=dtype), rnd(116, rows, n, dtype=dtype), 1 + 0.2 * rnd(117, n)
+    got = ops.rms_norm_quant(x, w, r, fmt="int8", normed=True)
+    h, v = norm_ref(x, w, r)
+    assert torch.equal(got.residual.double(), h)
+    within(got.normed, v, v.abs() * (32 * U + BF[dtype]))
+    check_quant(got.q, got.s, v, "int8", 32 * U)
+    gu = rnd(118, rows, 2 * n, dtype=dtype, scale=4.0)
+    q, s = ops.swiglu_quant(gu)
+    check_quant(q, s, swiglu_ref(gu), "int8", 16 * U)
+
+
 def test_rms_norm_quant_forms(ops):
     x, r, w = rnd(4, 2, 3, 256, dtype=torch.bfloat16), rnd(5, 2, 3, 256, dtype=torch.bfloat16), rnd(6, 256, dtype=torch.bfloat16)
     _, v = norm_ref(x, w, r, 0.1)
