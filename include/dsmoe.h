@@ -128,7 +128,8 @@ DSMOE_API int dsmoe_fp4_gemm(const void* a, int a_dtype, const float* a_s, long 
 DSMOE_API int dsmoe_act_quant(const void* x, int x_dtype, long long M, long long K, int block, int pow2,
                     uint8_t* q, float* s, void* stream);
 
-/* ---- 8-bit operators around the expert products ------------------------------------------- */
+/* ---- 8-bit operators around the expert products -------------------------------------------
+ * Outputs share no byte with an input or another output (DSMOE_ERR_ARG), except where it is said. */
 
 /* r = x + residual rounded to dtype (residual NULL: r = x), v = r / sqrt(mean(r^2) + eps) * weight per
  * row, v quantized: q_dtype DSMOE_DTYPE_E4M3 as in dsmoe_act_quant (one scale per 128 values, hidden a
@@ -136,7 +137,7 @@ DSMOE_API int dsmoe_act_quant(const void* x, int x_dtype, long long M, long long
  * s = max(amax, 1e-4) / 127, q = rint(v / s), s [rows]. residual_out (r; may be residual or x itself)
  * and normed (v rounded to dtype) may be NULL. dtype F32 or BF16, weight [hidden] F32 or BF16, hidden
  * <= 16384. Squares are summed in fp32; a row with an infinity or NaN, or whose squares overflow, gets NaN
- * scales. Pointers other than s are 16-byte aligned; q, s, residual_out and normed overlap nothing else.
+ * scales. Pointers other than s are 16-byte aligned.
  * Feeds dsmoe_fp8_gemm / dsmoe_int8_gemm. */
 DSMOE_API int dsmoe_rms_norm_quant(const void* x, int dtype, const void* residual, const void* weight, int w_dtype,
                                    long long rows, long long hidden, float eps, int q_dtype, int pow2, void* q, float* s,

@@ -18,6 +18,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/dsmoe.h"
 
 namespace dsmoe {
@@ -301,6 +303,25 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
 namespace dsmoe {
 void set_error(const char* fmt, ...);
 int cuda_status(const char* where);  // DSMOE_OK or DSMOE_ERR_CUDA after a launch
+
+// Whether an output shares a byte with an input or another output. Memory that is not there (p null) overlaps nothing.
+struct Mem {
+  const void* p;
+  long long bytes;
+};
+inline bool overlap(const Mem& a, const Mem& b) {
+  const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+  return x && y && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+inline bool overlap(std::initializer_list<Mem> outs, std::initializer_list<Mem> ins) {
+  for (const Mem* o = outs.begin(); o != outs.end(); ++o) {
+    for (const Mem* p = o + 1; p != outs.end(); ++p)
+      if (overlap(*o, *p)) return true;
+    for (const Mem& i : ins)
+      if (overlap(*o, i)) return true;
+  }
+  return false;
+}
 
 // A launch with programmatic dependent launch allowed: the kernel begins with pdl_wait.
 template <typename... P, typename... A>

@@ -774,6 +774,9 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   DSMOE_REQUIRE((((uintptr_t)a_s | (uintptr_t)b_s | (uintptr_t)offsets) & 3) == 0 &&
                     ((uintptr_t)out & (out_dtype == DSMOE_DTYPE_F32 ? 3 : 1)) == 0,
                 DSMOE_ERR_ALIGN, "%s: misaligned pointer", name);
+  DSMOE_REQUIRE(!overlap({{out, M * N * (out_dtype == DSMOE_DTYPE_F32 ? 4 : 2)}},
+                         {{x, M * K}, {a_s, M * 4}, {b, N * E * K}, {b_s, N * E * 4}, {offsets, (E + 1) * 4}}),
+                DSMOE_ERR_ARG, "%s: out overlaps an input", name);
   int sms = 0, optin = 0;
   int rc = device_limits(name, &sms, &optin);
   if (rc) return rc;

@@ -566,11 +566,6 @@ int run(Args& a, bool fp8, cudaStream_t st) {
   return cuda_status(NORM ? "rms_norm_quant" : "swiglu_quant");
 }
 
-bool overlap(const void* p, long long np, const void* q, long long nq) {
-  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
-  return p && q && a < b + (uintptr_t)nq && b < a + (uintptr_t)np;
-}
-
 int check(const char* name, int dtype, int q_dtype, int pow2, long long rows, long long n, const void* q, const float* s) {
   DSMOE_REQUIRE(q && s, DSMOE_ERR_ARG, "%s: null pointer", name);
   DSMOE_REQUIRE(dtype == DSMOE_DTYPE_F32 || dtype == DSMOE_DTYPE_BF16, DSMOE_ERR_ARG, "%s: dtype %d", name, dtype);
@@ -597,18 +592,16 @@ extern "C" int dsmoe_rms_norm_quant(const void* x, int dtype, const void* residu
   DSMOE_REQUIRE(w_dtype == DSMOE_DTYPE_F32 || w_dtype == DSMOE_DTYPE_BF16, DSMOE_ERR_ARG, "rms_norm_quant: w_dtype %d", w_dtype);
   DSMOE_REQUIRE(!residual_out || residual, DSMOE_ERR_ARG, "rms_norm_quant: residual_out without residual");
   const int sz = dtype == DSMOE_DTYPE_F32 ? 4 : 2;
-  // every output is its own memory; only residual_out may be x or residual themselves (element for element)
-  const long long nb = rows * hidden * sz;
-  DSMOE_REQUIRE((residual_out == residual || !rows8::overlap(residual_out, nb, residual, nb)) &&
-                    (residual_out == x || !rows8::overlap(residual_out, nb, x, nb)) &&
-                    !rows8::overlap(normed, nb, x, nb) && !rows8::overlap(normed, nb, residual, nb) &&
-                    !rows8::overlap(normed, nb, residual_out, nb) && !rows8::overlap(q, rows * hidden, x, nb) &&
-                    !rows8::overlap(q, rows * hidden, residual, nb) && !rows8::overlap(q, rows * hidden, residual_out, nb) &&
-                    !rows8::overlap(q, rows * hidden, normed, nb),
-                DSMOE_ERR_ARG, "rms_norm_quant: outputs overlap inputs");
   DSMOE_REQUIRE((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)residual_out | (uintptr_t)normed |
                   (uintptr_t)q) & 15) == 0 && ((uintptr_t)s & 3) == 0,
                 DSMOE_ERR_ALIGN, "rms_norm_quant: misaligned pointer");
+  // every output is its own memory; only residual_out may be x or residual themselves (element for element)
+  const long long nb = rows * hidden * sz, sb = (q_dtype == DSMOE_DTYPE_E4M3 ? rows * (hidden / 128) : rows) * 4;
+  DSMOE_REQUIRE(!overlap({{residual_out, nb}, {normed, nb}, {q, rows * hidden}, {s, sb}},
+                         {{x == residual_out ? nullptr : x, nb},
+                          {residual == residual_out ? nullptr : residual, nb},
+                          {weight, hidden * (w_dtype == DSMOE_DTYPE_F32 ? 4 : 2)}}),
+                DSMOE_ERR_ARG, "rms_norm_quant: outputs overlap inputs");
   rows8::Args a{};
   a.x = x; a.res = residual; a.w = weight; a.q = q; a.s = s; a.res_out = residual_out; a.normed = normed;
   a.rows = rows; a.n = (int)hidden; a.w_bf16 = w_dtype == DSMOE_DTYPE_BF16; a.pow2 = pow2; a.eps = eps;
@@ -626,7 +619,9 @@ extern "C" int dsmoe_swiglu_quant(const void* gu, int dtype, const float* row_we
   const int sz = dtype == DSMOE_DTYPE_F32 ? 4 : 2;
   DSMOE_REQUIRE((((uintptr_t)gu | (uintptr_t)q) & 15) == 0 && (((uintptr_t)s | (uintptr_t)row_weight) & 3) == 0, DSMOE_ERR_ALIGN,
                 "swiglu_quant: misaligned pointer");
-  DSMOE_REQUIRE(!rows8::overlap(q, rows * inter, gu, 2 * rows * inter * sz), DSMOE_ERR_ARG, "swiglu_quant: q overlaps gu");
+  const long long sb = (q_dtype == DSMOE_DTYPE_E4M3 ? rows * (inter / 128) : rows) * 4;
+  DSMOE_REQUIRE(!overlap({{q, rows * inter}, {s, sb}}, {{gu, 2 * rows * inter * sz}, {row_weight, rows * 4}}), DSMOE_ERR_ARG,
+                "swiglu_quant: outputs overlap inputs");
   rows8::Args a{};
   a.x = gu; a.w = row_weight; a.q = q; a.s = s; a.rows = rows; a.n = (int)inter; a.pow2 = pow2; a.limit = limit;
   const bool fp8 = q_dtype == DSMOE_DTYPE_E4M3;

@@ -446,6 +446,9 @@ extern "C" int dsmoe_sort_tokens(const int64_t* idx, long long P, int k, int n_e
   DSMOE_REQUIRE(idx && pos && src && offsets, DSMOE_ERR_ARG, "sort_tokens: null pointer");
   DSMOE_REQUIRE(((uintptr_t)idx & 7) == 0 && (((uintptr_t)pos | (uintptr_t)src | (uintptr_t)offsets) & 3) == 0, DSMOE_ERR_ALIGN,
                 "sort_tokens: misaligned pointer");
+  const long long pairs = P * k;
+  DSMOE_REQUIRE(!overlap({{pos, pairs * 4}, {src, pairs * 4}, {offsets, (n_experts + 1) * 4}}, {{idx, pairs * 8}}), DSMOE_ERR_ARG,
+                "sort_tokens: outputs overlap");
   tokens::SortArgs a{idx, pos, src, offsets, (int)(P * k), n_experts, 0, 0};
   // 131072 pairs of 384 experts: 26.8 us with 8 CTAs, 16.9 with 16 (24576 pairs 8.1 and 6.3; 12282: 6.5 and 6.6)
   const int C = a.n > 16384 && tokens::sixteen() ? 16 : a.n > 4096 ? 8 : 1;
@@ -484,6 +487,9 @@ extern "C" int dsmoe_dispatch_rows(const void* x, const float* s, const int* pos
   DSMOE_REQUIRE(row_bytes > 0 && row_bytes < (1LL << 31), DSMOE_ERR_ARG, "dispatch_rows: row of %lld bytes", row_bytes);
   DSMOE_REQUIRE((((uintptr_t)pos | (uintptr_t)offsets | (uintptr_t)s | (uintptr_t)ss) & 3) == 0, DSMOE_ERR_ALIGN,
                 "dispatch_rows: misaligned pointer");
+  DSMOE_REQUIRE(!overlap({{xs, P * k * row_bytes}, {ss, P * k * 4}},
+                         {{x, P * row_bytes}, {s, P * 4}, {pos, P * k * 4}, {offsets, (n_experts + 1) * 4}}),
+                DSMOE_ERR_ARG, "dispatch_rows: outputs overlap inputs");
   cudaStream_t st = (cudaStream_t)stream;
   const uintptr_t any = (uintptr_t)x | (uintptr_t)xs | (uintptr_t)row_bytes;
   if ((any & 15) == 0) tokens::dispatch<uint4>(x, s, pos, offsets, n_experts, P, k, row_bytes, xs, ss, st);
@@ -504,6 +510,8 @@ extern "C" int dsmoe_combine_rows(const void* ys, int dtype, const int* pos, con
   const uintptr_t any = (uintptr_t)ys | (uintptr_t)y;
   DSMOE_REQUIRE((any & (sz - 1)) == 0 && (((uintptr_t)pos | (uintptr_t)wt) & 3) == 0, DSMOE_ERR_ALIGN,
                 "combine_rows: misaligned pointer");
+  DSMOE_REQUIRE(!overlap({{y, P * width * sz}}, {{ys, P * k * width * sz}, {pos, P * k * 4}, {wt, P * k * 4}}), DSMOE_ERR_ARG,
+                "combine_rows: y overlaps an input");
   const bool wide = ((any | (uintptr_t)(width * sz)) & 15) == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DSMOE_DTYPE_F32) tokens::combine<float>(ys, pos, wt, P, k, width, wide, y, st);
@@ -523,6 +531,10 @@ extern "C" int dsmoe_combine_grad(const void* dy, const void* ys, int dtype, con
   DSMOE_REQUIRE((any & (sz - 1)) == 0 &&
                     (((uintptr_t)pos | (uintptr_t)wt | (uintptr_t)offsets | (uintptr_t)dwt) & 3) == 0,
                 DSMOE_ERR_ALIGN, "combine_grad: misaligned pointer");
+  const long long nb = P * width * sz;
+  DSMOE_REQUIRE(!overlap({{dys, nb * k}, {dwt, P * k * 4}},
+                         {{dy, nb}, {ys, nb * k}, {pos, P * k * 4}, {wt, P * k * 4}, {offsets, (n_experts + 1) * 4}}),
+                DSMOE_ERR_ARG, "combine_grad: outputs overlap inputs");
   const bool wide = ((any | (uintptr_t)(width * sz)) & 15) == 0;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == DSMOE_DTYPE_F32)

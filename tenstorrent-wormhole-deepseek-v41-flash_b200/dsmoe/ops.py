@@ -67,9 +67,9 @@ def swiglu_quant(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, *,
 def int8_gemm(a: torch.Tensor, a_s: torch.Tensor, b: torch.Tensor, b_s: torch.Tensor, out_dtype=None,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """(a @ b^T) * a_s * b_s: a [..., K] int8 with one scale per token (a_s [...]), b [N, K] int8 with one per
-    channel (b_s [N]), beside ``fp8_gemm`` / ``fp4_gemm``. The integer sum is exact; the product with the
-    scales is rounded once to ``out_dtype`` (default: the default dtype, as there; bf16 or fp32). K is a
-    multiple of 16, at most 131071."""
+    channel (b_s [N]), beside ``fp8_gemm`` / ``fp4_gemm``. The integer sum is exact; it is taken to fp32, times
+    b_s, times a_s, and rounded to ``out_dtype`` (default: the default dtype, as there; bf16 or fp32). K is a
+    multiple of 16, at most 131071. ``out``: contiguous, sharing no memory with the inputs."""
     return _ops.int8_product(a, a_s, b, b_s, None, out_dtype, out)
 
 

@@ -80,6 +80,33 @@ def test_token_entry_points_refuse():
         assert _code("dsmoe_combine_grad", *{**grad, **change}.values()) == code, change
 
 
+def test_outputs_are_their_own_memory():
+    """One byte in common is enough, whichever end; neighbours are fine as far as this check goes."""
+    norm, gemm = {**NORM, "residual_out": 2 * A}, {**GROUPED, "out": 5 * A}
+    for name, args, change in (
+            ("dsmoe_rms_norm_quant", norm, dict(weight=2 * A + 2032)), ("dsmoe_rms_norm_quant", norm, dict(s=3 * A + 1020)),
+            ("dsmoe_rms_norm_quant", norm, dict(s=A - 28)), ("dsmoe_rms_norm_quant", norm, dict(s=4 * A)),
+            ("dsmoe_swiglu_quant", SWIGLU, dict(row_weight=8 * A + 28)), ("dsmoe_swiglu_quant", SWIGLU, dict(s=A + 4092)),
+            ("dsmoe_int8_gemm", GEMM, dict(out=A + 254)), ("dsmoe_int8_gemm", GEMM, dict(out=2 * A - 254)),
+            ("dsmoe_int8_gemm", GEMM, dict(out=3 * A + 2046)), ("dsmoe_int8_gemm", GEMM, dict(out=4 * A + 126)),
+            ("dsmoe_int8_grouped_gemm", gemm, dict(out=3 * A + 6142)), ("dsmoe_int8_grouped_gemm", gemm, dict(out=6 * A + 14)),
+            ("dsmoe_int8_grouped_gemm", gemm, dict(out=4 * A + 382))):
+        assert _code(name, *{**args, **change}.values()) == -1, (name, change)
+    sort = dict(idx=A, P=4, k=2, n_experts=8, pos=2 * A, src=3 * A, offsets=4 * A, stream=None)
+    disp = dict(x=A, s=5 * A, pos=2 * A, offsets=3 * A, n_experts=8, P=4, k=2, row_bytes=64, xs=4 * A, ss=6 * A, stream=None)
+    comb = dict(ys=A, dtype=1, pos=2 * A, wt=4 * A, P=4, k=2, width=64, y=3 * A, stream=None)
+    grad = dict(dy=A, ys=2 * A, dtype=1, pos=3 * A, wt=4 * A, offsets=5 * A, n_experts=8, P=4, k=2, width=64, dys=6 * A,
+                dwt=7 * A, stream=None)
+    for name, args, change in (
+            ("dsmoe_sort_tokens", sort, dict(pos=A + 60)), ("dsmoe_sort_tokens", sort, dict(src=2 * A + 28)),
+            ("dsmoe_sort_tokens", sort, dict(offsets=A - 32)), ("dsmoe_dispatch_rows", disp, dict(xs=A + 240)),
+            ("dsmoe_dispatch_rows", disp, dict(ss=4 * A + 508)), ("dsmoe_dispatch_rows", disp, dict(ss=5 * A + 12)),
+            ("dsmoe_combine_rows", comb, dict(y=A + 1008)), ("dsmoe_combine_rows", comb, dict(y=4 * A + 28)),
+            ("dsmoe_combine_grad", grad, dict(dys=A + 496)), ("dsmoe_combine_grad", grad, dict(dys=2 * A - 1008)),
+            ("dsmoe_combine_grad", grad, dict(dwt=6 * A + 1020)), ("dsmoe_combine_grad", grad, dict(dwt=5 * A + 32))):
+        assert _code(name, *{**args, **change}.values()) == -1, (name, change)
+
+
 def test_python_surface_takes_cuda_tensors_only():
     import dsmoe
     x, w = torch.zeros(2, 128), torch.ones(128)
