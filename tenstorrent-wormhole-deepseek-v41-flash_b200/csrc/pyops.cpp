@@ -104,6 +104,10 @@ Tensor dense(const Tensor& t, bool aligned = true) {
   return aligned && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
 }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// A caller's tensor that a kernel writes: autograd refuses a backward pass that saved what stood there.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // The call on t's device and that device's current stream.
 template <typename F>
@@ -197,7 +201,8 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return dsmoe_rms_norm_quant(ptr(x), dt, ptr(r), ptr(w), wdt, x.numel() / h, h, static_cast<float>(eps), code, pow2,
                                     ptr(q), static_cast<float*>(ptr(s)), ptr(out), ptr(y), st);
       });
-      if (inplace && out.data_ptr() != r0.data_ptr()) r0.copy_(out);  // it was not 16-byte aligned
+      if (inplace && out.data_ptr() == r0.data_ptr()) written(r0);
+      else if (inplace) r0.copy_(out);  // it was not 16-byte aligned
     }
     return tuple({&q, &s, inplace ? &r0 : &out, &y});
   });
@@ -274,6 +279,7 @@ PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (!out.defined()) out = empty(a0, shape, dt);
     const int64_t M = a0.numel() / K;
     if (M && N) {
+      if (args[6] != Py_None) written(out);
       const Tensor a = dense(a0), b = dense(b0), as = dense(as0, false), bs = dense(bs0, false);
       const int code = dt == at::kFloat ? DSMOE_DTYPE_F32 : DSMOE_DTYPE_BF16;
       run(a, [&](void* st) {

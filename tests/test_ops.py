@@ -142,6 +142,24 @@ def test_rms_norm_quant_forms(ops):
     check_quant(twice.q, twice.s, norm_ref(x, w, x)[1], "int8", 32 * U)
 
 
+def test_written_tensors_are_known_to_autograd(ops):
+    x, w = rnd(119, 3, 256), torch.ones(256, device="cuda")
+    a, b, sa, sb = codes(120, 3, 64), codes(121, 256, 64), scales(122, 3), scales(123, 256)
+    for r in (rnd(124, 3, 256), torch.zeros(769, device="cuda")[1:].view(3, 256)):
+        leaf = rnd(125, 3, 256).requires_grad_()
+        for write in (lambda: ops.rms_norm_quant(x, w, r, inplace=True), lambda: ops.int8_gemm(a, sa, b, sb, out=r)):
+            y, before = (leaf * r).sum(), r._version
+            write()
+            assert r._version > before
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+    with torch.inference_mode():
+        r, out = rnd(124, 3, 256), torch.empty(3, 256, device="cuda")
+        want = ops.int8_gemm(a, sa, b, sb)
+    ops.rms_norm_quant(x, w, r, inplace=True)
+    assert torch.equal(r, x + rnd(124, 3, 256)) and torch.equal(ops.int8_gemm(a, sa, b, sb, out=out), want)
+
+
 @pytest.mark.parametrize("fmt", ["fp8", "int8"])
 def test_rms_norm_quant_special_rows(ops, fmt):
     x, w = rnd(7, 6, 256, dtype=torch.bfloat16), torch.ones(256, device="cuda")
