@@ -321,6 +321,46 @@ def test_int8_grouped_gemm(ops, counts, n, k, tail, dtype):
     assert not out[at:].any()
 
 
+# more tiles than the pairs of CTAs of the GPU, of one and of two halves; tails: rows behind the last group
+BIG_GROUPS = [([3000, 1, 2000, 0, 2999], 2100, 272, 0), ([1, 5000, 300], 4096, 16, 0), ([700, 513, 0, 33, 4000, 90], 3000, 640, 77),
+              ([257] * 16, 1030, 144, 0), ([12000], 700, 48, 0), ([200, 4000, 1, 1500], 4100, 1040, 6000), ([40, 9], 4096, 64, 8000),
+              ([0, 0, 0], 1500, 32, 9000), ([129] * 70, 640, 16, 1), ([1000, 31] * 12, 2304, 208, 0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("counts,n,k,tail", BIG_GROUPS)
+def test_int8_grouped_gemm_many_tiles(ops, counts, n, k, tail, dtype):
+    test_int8_grouped_gemm(ops, counts, n, k, tail, dtype)
+
+
+def test_int8_grouped_gemm_many_tiles_at_once(ops):
+    """Two streams and a graph of calls in a row; offsets that describe no groups in the same shapes."""
+    sets = []
+    for i, counts in enumerate(([3000, 1, 2000, 0, 2999], [0, 8000, 0, 0, 0], [1, 2, 3, 4, 100])):
+        off = group_offsets(counts)
+        t = codes(130 + i, 8000, 272), scales(131 + i, 8000), codes(132 + i, 5, 2100, 272), scales(133 + i, 5, 2100), off
+        sets.append((t, ops.int8_grouped_gemm(*t)))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(12):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append(ops.int8_grouped_gemm(*sets[i % 3][0]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, sets[i % 3][1]) for i, g in enumerate(got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = [ops.int8_grouped_gemm(*sets[i % 3][0]) for i in range(7)]
+    for _ in range(3):
+        for o in out:
+            o.fill_(7.0)
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, sets[i % 3][1]) for i, o in enumerate(out))
+    (a, sa, b, sb, _), _ = sets[0]
+    for bad in ([0, 5, 3, 8, 8, 8], [0, 1, 2, 3, 4, 8001], [1, 1, 1, 1, 1, 8000]):
+        assert bool(torch.isnan(ops.int8_grouped_gemm(a, sa, b, sb, torch.tensor(bad, dtype=torch.int32, device="cuda"))).all()), bad
+
+
 def test_int8_grouped_gemm_bad_offsets(ops):
     a, b, sa, sb = codes(23, 8, 64), codes(24, 3, 40, 64), scales(25, 8), scales(26, 3, 40)
     for bad in ([0, 5, 3, 8], [1, 2, 3, 8], [0, 4, 6, 9], [0, -1, 4, 8], [-5, 0, 0, 0], [0, 2 ** 30, 2 ** 31 - 1, 8]):
