@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 
@@ -710,22 +711,59 @@ int one_tile_stages(int TT, int kb, size_t tables, size_t optin) {
   return std::min(std::max(std::min(kb, 4), need), (int)((optin - tables) / SB));
 }
 
+// Tensor memory columns of a one-tile CTA.
+unsigned tile_columns(int TT) { return TT <= 32 ? 32 : TT <= 64 ? 64 : TT <= 128 ? 128 : 256; }
+
+// Groups: their sizes are known to the device alone, so the model takes popularities that fall like rank^-1.1: G
+// experts are reached, and tiles of TT tokens number 1.4 for each and one per TT rows. A tile costs its set-up, its K
+// blocks (latency, or the bytes an SM takes in) and its store; tiles beyond what the GPU holds at once queue, and so do
+// the CTAs of tiles that could have been there; the weights that are reached come from memory. Constants fitted to 227
+// cases (1 to 24576 rows, 4 to 384 experts, N 64 to 5120, K 64 to 5120): on the mean 3 % over the best shape of each,
+// where a tile of 16 or 32 tokens for up to 64 rows and pairs for more was 17 % (456 rows of 6 experts, N 121, K 2960:
+// pairs 13.2 us, 32 x 8 CTAs 7.2; 4285 of 10, N 332, K 112: 11.0, 32 x 1 6.0; 48 of 384, N 512, K 5120: 33, 64 x 2 18.6,
+// 16 x 1 21.1). A wider tile must gain 1.5 %, as sizes are not known; pairs on 512 tokens, which are stored before the
+// next tile begins, want the mean group to fill half of them (24576 of 64 x 4096 x 5120: 501, 502 with 256; of 384 x 512
+// x 5120: 218, 198).
+Plan plan_groups(long long M, long long N, int nkb, int E, int sms, size_t tables, size_t optin) {
+  const double G = std::min<double>((double)M * E / (M + 1.15 * E - 0.15), std::min<long long>(E, M)), mem = G * N * nkb * 128 / 6.2e6 + M * N * 2 / 6.2e6;
+  auto total = [&](double x, double start) {
+    return start + std::sqrt(std::sqrt(x * x * x * x + mem * mem * mem * mem));
+  };
+  Plan best{false, 16, 1};
+  double least = 1e30;
+  for (int TT = 16; TT <= 256 && (TT == 16 || TT < 2 * M); TT *= 2) {
+    const double m = 1.4 * G + (double)M / TT, cols = std::min<double>(TT, M / m), ntn = (N + TM - 1) / TM;
+    double t = 1e30;
+    int at = 1;
+    for (int S = 1; S <= 8 && S <= nkb; S *= 2) {
+      const int kb = (nkb + S - 1) / S;
+      const size_t ring = tables + (size_t)one_tile_stages(TT, kb, tables, optin) * (TM + TT) * 128;
+      const size_t smem = S > 1 ? std::max(ring, kHalfSmem) : ring;
+      const int occ = std::min({(int)((optin + 1024) / (smem + 1024)), 3, (int)(512 / tile_columns(TT))});
+      const double fit = (S == 8 ? sms * 13 / 15 : S == 4 ? sms * 14 / 15 : sms) * occ, queue = m * ntn * S / fit;
+      const double idle = ntn * S * (M / TT + std::min<long long>(E, M)) / fit - std::max(1.0, queue);
+      const double block = std::max(0.33, std::max(1.0, occ * std::min(1.0, queue)) * (TM + cols) * 128 / 105e3);
+      const double u = total(std::max(1.0, queue) * (3.7 + kb * block + (S > 1 ? 0.033 : 0.0183) * cols) + 4.0 * std::max(0.0, idle), 2.2);
+      if (u < t) t = u, at = S;
+    }
+    if (t < 0.985 * least) least = t, best = Plan{false, TT, at};
+  }
+  for (int TT = 128; TT <= (M < 256LL * E ? 256 : PTT); TT *= 2) {
+    const double m = 1.4 * G + (double)M / TT, cols = std::min<double>(TT, M / m), store = 0.0113 * cols;
+    const double blocks = nkb * std::max(0.00105 * cols, (TM * 128 + cols / 2 * 128) / 105e3);
+    const double queue = m * ((N + 2 * TM - 1) / (2 * TM)) / (sms / 2);
+    const double t = total(std::max(1.0, queue) * (1.45 + (TT > 256 ? blocks + store : std::max(blocks, 1.2 * store))), 6.2);
+    if (t < 0.985 * least) least = t, best = Plan{true, TT, 2};
+  }
+  return best;
+}
+
 // The tile shape that should take least time, in us, by a model of what bounds each kernel, its constants fitted to
 // measurements on a B200 (M 1..4096, N 72..8192, K 64..8192). An SM takes in at most 105 bytes/ns, and no more than its
 // ring's bytes in a round trip (2.2 us for weights that come from memory, 1.4 where other tiles brought them to L2);
 // all weights come from memory at 6200 bytes/ns; a K block takes 0.33 us, 0.34 in a pair.
 Plan plan(long long M, long long N, int nkb, int E, int sms, size_t tables, size_t optin) {
-  if (E) {
-    // Groups: sizes are known to the device alone. Few rows: every expert has few, one tile each, K shared by two or
-    // four CTAs while the tiles cannot fill the GPU (48 rows of 384 experts, N 512: S = 1 20.9 us, 2 19.2; 6 rows: 2
-    // 12.6, 4 9.3). Else pairs, which adapt a tile's width to its group (384 rows: 65.8 us, one-tile 64.2; 6144 rows:
-    // 165 and 172; 8000 rows of 8 experts 87 and 118): up to 128, 256 or 512 tokens by the mean group.
-    if (M > 64) return Plan{true, M < 32LL * E ? 128 : M < 256LL * E ? 256 : PTT, 2};
-    const long long tiles = (N + TM - 1) / TM * (M / 32 + std::min<long long>(E, M));
-    int S = 1;
-    while (S < 4 && S * 2 <= nkb && tiles * S * 2 <= 400) S *= 2;
-    return Plan{false, M <= 16 ? 16 : 32, S};
-  }
+  if (E) return plan_groups(M, N, nkb, E, sms, tables, optin);
   Plan best{false, 16, 1};
   double least = 1e30;
   const double weights = (double)N * nkb * 128 / 6.2e6;
@@ -804,7 +842,7 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
     a.RS = std::min(MAXRS, (int)((optin - tables) / SB));
   } else {
     a.RS = one_tile_stages(a.TT, (a.nkb + p.S - 1) / p.S, tables, optin);
-    a.tcols = a.TT <= 32 ? 32 : a.TT <= 64 ? 64 : a.TT <= 128 ? 128 : 256;
+    a.tcols = tile_columns(a.TT);
   }
   // Shared memory also decides who shares an SM, and with it its tensor memory, whose allocation waits without a limit
   // while CTAs of a cluster wait for one another. A pair (all 512 columns) takes the whole SM; a CTA of a cluster half of

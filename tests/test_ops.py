@@ -333,6 +333,21 @@ def test_int8_grouped_gemm_many_tiles(ops, counts, n, k, tail, dtype):
     test_int8_grouped_gemm(ops, counts, n, k, tail, dtype)
 
 
+# rows, n, k, experts: from one row to thousands, few and many K blocks, every width of tile and split of K
+SPREAD_GROUPS = [(1, 96, 1136, 2), (405, 700, 16, 40), (176, 257, 144, 40), (34, 130, 592, 40), (32, 96, 944, 40), (912, 700, 16, 40),
+                 (43, 400, 496, 40), (35, 96, 1568, 40), (293, 257, 144, 40), (86, 130, 1312, 40), (75, 257, 928, 8),
+                 (1391, 1500, 400, 5), (1947, 130, 1312, 40), (456, 121, 2960, 6), (324, 155, 1168, 6), (1437, 81, 3680, 146)]
+
+
+@pytest.mark.parametrize("skew", [0.0, 1.1, 4.0])
+@pytest.mark.parametrize("rows,n,k,e", SPREAD_GROUPS)
+def test_int8_grouped_gemm_spreads(ops, rows, n, k, e, skew):
+    g = torch.Generator().manual_seed(rows)
+    p = torch.arange(1, e + 1, dtype=torch.float64)[torch.randperm(e, generator=g)] ** -skew
+    counts = torch.bincount(torch.multinomial(p, rows, replacement=True, generator=g), minlength=e).tolist()
+    test_int8_grouped_gemm(ops, counts, n, k, 0 if skew else 5, torch.bfloat16 if skew else torch.float32)
+
+
 def test_int8_grouped_gemm_many_tiles_at_once(ops):
     """Two streams and a graph of calls in a row; offsets that describe no groups in the same shapes."""
     sets = []
