@@ -13,7 +13,7 @@
 // Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.6 us (5.8 TB/s; a copy of those bytes
 // 28.9), one row 2.3 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.2 us to e4m3 (5.2 TB/s; 19.3), 26.0 to int8:
 // about 22 instructions a value keep the issue slots two thirds busy. Rows that are not a multiple of 16 bytes cost
-// shifts and masks: 6000 x 2049 23.6 us (2.6 TB/s).
+// shifts and masks: swiglu of 6000 x 2049 to int8 23.6 us (2.6 TB/s), norm of 4000 x 6387 with residual 54.9 (3.3).
 // Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
 // or NaN or whose squares overflow fp32, and of a swiglu's row (e4m3: block) whose amax is not finite.
 #include "common.cuh"
@@ -56,16 +56,20 @@ struct Raw<__nv_bfloat16> {
       if (i < n) w[i >> 1] |= (uint32_t)h[i] << (16 * (i & 1));
     u = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // values s.. of this chunk followed by the next one's (0 <= s < 8, the same in every lane of a row)
+  // values s.. of this chunk followed by the next one's (0 < s < 8, the same in every lane of a row)
   __device__ __forceinline__ void shift_in(const Raw& next, int s) {
-    uint32_t w[8] = {u.x, u.y, u.z, u.w, next.u.x, next.u.y, next.u.z, next.u.w};
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = s & 4 ? w[i + 2] : w[i];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = s & 2 ? w[i + 1] : w[i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = s & 1 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
-    u = make_uint4(w[0], w[1], w[2], w[3]);
+    const uint4 n = next.u;
+    switch (s >> 1) {
+      case 0: words(u.x, u.y, u.z, u.w, n.x, s); break;
+      case 1: words(u.y, u.z, u.w, n.x, n.y, s); break;
+      case 2: words(u.z, u.w, n.x, n.y, n.z, s); break;
+      default: words(u.w, n.x, n.y, n.z, n.w, s); break;
+    }
+  }
+  __device__ __forceinline__ void words(uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, int s) {
+    const int half = (s & 1) * 16;
+    u = make_uint4(__funnelshift_r(a, b, half), __funnelshift_r(b, c, half), __funnelshift_r(c, d, half),
+                   __funnelshift_r(d, e, half));
   }
   __device__ __forceinline__ void get(float (&o)[8]) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -552,11 +556,13 @@ int run(Args& a, bool fp8, cudaStream_t st) {
   const bool edge = a.n % V != 0;
   const int nchunk = edge ? (a.n - 2) / V + 2 : a.n / V;  // a row's chunks, at most
   // Chunks per thread: one, so that a row's loads go out at once from many threads. The norm's fixed work per thread
-  // is worth two where the grid fills the GPU several times (4096 rows of 5120 32.7 us, 34.7 with one); with an edge
-  // one is as fast, and the swiglu loses (12282 rows of 2048 24.2 us, 27.6 with two). A row keeps 32 threads.
+  // is worth two where the grid fills the GPU several times (4096 rows of 5120 32.7 us, 34.7 with one), and with an
+  // edge, where registers let few threads onto an SM, from about one long row per SM on (4000 rows of 6387 54.9 us, 86.6
+  // with one; 160: 4.7, 6.2; but 100 of 5001 3.6, 3.1, and 400 of 1501 3.9, 3.3). The swiglu loses (12282 rows of 2048
+  // 24.2 us, 27.6 with two; 6000 of 2049 23.6, 26.0). A row keeps 32 threads.
   int nv = 1;
   while ((nchunk + nv - 1) / nv > 1024) nv *= 2;
-  if (NORM && !edge && nv == 1 && nchunk >= 64 && a.rows * nchunk >= 8192LL * sm_count()) nv = 2;
+  if (NORM && nv == 1 && nchunk >= (edge ? 128 : 64) && a.rows * nchunk >= (edge ? 600LL : 8192LL) * sm_count()) nv = 2;
   a.tpr = ((nchunk + nv - 1) / nv + 31) / 32 * 32;
   a.rpc = a.tpr >= 256 ? 1 : 256 / a.tpr;
   if (a.rpc > a.rows) a.rpc = (int)a.rows;
