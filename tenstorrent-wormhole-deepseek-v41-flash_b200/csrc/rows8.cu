@@ -13,7 +13,7 @@
 // Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.6 us (5.8 TB/s; a copy of those bytes
 // 28.9), one row 2.3 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.2 us to e4m3 (5.2 TB/s; 19.3), 26.0 to int8:
 // about 22 instructions a value keep the issue slots two thirds busy. Rows that are not a multiple of 16 bytes cost
-// shifts and masks: swiglu of 6000 x 2049 to int8 23.6 us (2.6 TB/s), norm of 4000 x 6387 with residual 54.9 (3.3).
+// shifts and masks: swiglu of 6000 x 2049 to int8 22.7 us (2.7 TB/s), norm of 4000 x 6387 with residual 54.9 (3.3).
 // Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
 // or NaN or whose squares overflow fp32, and of a swiglu's row (e4m3: block) whose amax is not finite.
 #include "common.cuh"
@@ -56,7 +56,7 @@ struct Raw<__nv_bfloat16> {
       if (i < n) w[i >> 1] |= (uint32_t)h[i] << (16 * (i & 1));
     u = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  // values s.. of this chunk followed by the next one's (0 < s < 8, the same in every lane of a row)
+  // values s.. of this chunk followed by the next one's (0 <= s < 8, the same in every lane of a row)
   __device__ __forceinline__ void shift_in(const Raw& next, int s) {
     const uint4 n = next.u;
     switch (s >> 1) {
@@ -498,9 +498,20 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
     y[j].zero();
     if (p.hi) {
       if constexpr (EDGE) {  // the codes' chunks are aligned; g and u lie at their own offsets to them
-        const bool inner = (a.rows - 1 - row) * a.n >= VEC;  // 2 VEC values: a span is two chunks
-        x[j] = load_any(gu, e, total, inner);
-        y[j] = load_any(gu, e + a.n, total, inner);
+        if ((a.rows - 1 - row) * a.n >= VEC) {  // 2 VEC values behind the row: two whole chunks lie inside
+          const long long eg = 2 * row * a.n - (row * a.n & (VEC - 1)), eu = eg + a.n;  // where the row's chunk 0 begins
+          const int sg = (int)(eg & (VEC - 1)), su = (int)(eu & (VEC - 1)), c = (j * a.tpr + t) * VEC;
+          Raw<T> xn, yn;
+          x[j].load(gu + (eg - sg) + c);
+          xn.load(gu + (eg - sg) + c + VEC);
+          y[j].load(gu + (eu - su) + c);
+          yn.load(gu + (eu - su) + c + VEC);
+          x[j].shift_in(xn, sg);
+          y[j].shift_in(yn, su);
+        } else {
+          x[j] = load_any(gu, e, total, false);
+          y[j] = load_any(gu, e + a.n, total, false);
+        }
       } else {
         x[j].load(gu + e);
         y[j].load(gu + e + a.n);
@@ -559,7 +570,7 @@ int run(Args& a, bool fp8, cudaStream_t st) {
   // is worth two where the grid fills the GPU several times (4096 rows of 5120 32.7 us, 34.7 with one), and with an
   // edge, where registers let few threads onto an SM, from about one long row per SM on (4000 rows of 6387 54.9 us, 86.6
   // with one; 160: 4.7, 6.2; but 100 of 5001 3.6, 3.1, and 400 of 1501 3.9, 3.3). The swiglu loses (12282 rows of 2048
-  // 24.2 us, 27.6 with two; 6000 of 2049 23.6, 26.0). A row keeps 32 threads.
+  // 24.2 us, 27.6 with two; 6000 of 2049 22.7, 26.0). A row keeps 32 threads.
   int nv = 1;
   while ((nchunk + nv - 1) / nv > 1024) nv *= 2;
   if (NORM && nv == 1 && nchunk >= (edge ? 128 : 64) && a.rows * nchunk >= (edge ? 600LL : 8192LL) * sm_count()) nv = 2;
