@@ -13,7 +13,7 @@
 // Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.6 us (5.8 TB/s; a copy of those bytes
 // 28.9), one row 2.3 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.2 us to e4m3 (5.2 TB/s; 19.3), 26.0 to int8:
 // about 22 instructions a value keep the issue slots two thirds busy. Rows that are not a multiple of 16 bytes cost
-// shifts and masks: swiglu of 6000 x 2049 to int8 22.7 us (2.7 TB/s), norm of 4000 x 6387 with residual 54.9 (3.3).
+// shifts and masks: swiglu of 6000 x 2049 to int8 22.7 us (2.7 TB/s), norm of 4000 x 6387 with residual 50.9 (3.5).
 // Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
 // or NaN or whose squares overflow fp32, and of a swiglu's row (e4m3: block) whose amax is not finite.
 #include "common.cuh"
@@ -179,35 +179,70 @@ __device__ __forceinline__ float round_to(float v) {
   else return v;
 }
 
-// weights of VEC consecutive channels from k on, fp32 or bf16; EDGE: any k, zeros outside the row
-template <int VEC, bool EDGE>
+// weights of VEC consecutive channels from k on, fp32 or bf16
+template <int VEC>
 __device__ __forceinline__ void load_w(const Args& a, int k, float (&v)[VEC]) {
   if (a.w_bf16) {
     const __nv_bfloat16* w = reinterpret_cast<const __nv_bfloat16*>(a.w);
-    if constexpr (EDGE) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(w + k);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = k + i >= 0 && k + i < a.n ? (float)w[k + i] : 0.f;
-    } else {
-      const uint32_t* p = reinterpret_cast<const uint32_t*>(w + k);
-#pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) {
-        const uint32_t u = p[i];
-        v[2 * i] = __uint_as_float(u << 16);
-        v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
-      }
+    for (int i = 0; i < VEC / 2; ++i) {
+      const uint32_t u = p[i];
+      v[2 * i] = __uint_as_float(u << 16);
+      v[2 * i + 1] = __uint_as_float(u & 0xFFFF0000u);
     }
   } else {
     const float* w = reinterpret_cast<const float*>(a.w);
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i) {
       Raw<float> u;
-      if constexpr (EDGE) u = load_any<float>(w, k + 4 * i, a.n, k >= 8 && k + 16 <= a.n);
-      else u.load(w + k + 4 * i);
+      u.load(w + k + 4 * i);
       float f[4];
       u.get(f);
 #pragma unroll
       for (int q = 0; q < 4; ++q) v[4 * i + q] = f[q];
     }
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void take(const float (&f)[VEC + 4], int s, float (&v)[VEC]) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = f[i + s];
+}
+// ... from any k on, zeros outside the row: aligned groups of 4, shifted by a branch that a whole row takes alike
+template <int VEC>
+__device__ __forceinline__ void load_w_any(const Args& a, int k, float (&v)[VEC]) {
+  const __nv_bfloat16* wb = reinterpret_cast<const __nv_bfloat16*>(a.w);
+  const float* w = reinterpret_cast<const float*>(a.w);
+  if (k < 8 || k + 16 > a.n) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = k + i < 0 || k + i >= a.n ? 0.f : a.w_bf16 ? (float)wb[k + i] : w[k + i];
+    return;
+  }
+  const int s = k & 3;
+  float f[VEC + 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4 + 1; ++i) {
+    if (a.w_bf16) {
+      const uint2 u = *reinterpret_cast<const uint2*>(wb + k - s + 4 * i);
+      f[4 * i] = __uint_as_float(u.x << 16);
+      f[4 * i + 1] = __uint_as_float(u.x & 0xFFFF0000u);
+      f[4 * i + 2] = __uint_as_float(u.y << 16);
+      f[4 * i + 3] = __uint_as_float(u.y & 0xFFFF0000u);
+    } else {
+      const float4 u = *reinterpret_cast<const float4*>(w + k - s + 4 * i);
+      f[4 * i] = u.x;
+      f[4 * i + 1] = u.y;
+      f[4 * i + 2] = u.z;
+      f[4 * i + 3] = u.w;
+    }
+  }
+  switch (s) {
+    case 0: take<VEC>(f, 0, v); break;
+    case 1: take<VEC>(f, 1, v); break;
+    case 2: take<VEC>(f, 2, v); break;
+    default: take<VEC>(f, 3, v); break;
   }
 }
 
@@ -353,7 +388,8 @@ __device__ __forceinline__ void norm_row(const Args& a, const Raw<T> (&x)[NV], c
         if (i < p.lo || i >= p.hi) v[j][i] = 0.f;  // the neighbouring rows' values
     }
     float w[VEC];
-    load_w<VEC, EDGE>(a, p.k, w);
+    if constexpr (EDGE) load_w_any<VEC>(a, p.k, w);
+    else load_w<VEC>(a, p.k, w);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       sum = fmaf(v[j][i], v[j][i], sum);
@@ -568,8 +604,8 @@ int run(Args& a, bool fp8, cudaStream_t st) {
   const int nchunk = edge ? (a.n - 2) / V + 2 : a.n / V;  // a row's chunks, at most
   // Chunks per thread: one, so that a row's loads go out at once from many threads. The norm's fixed work per thread
   // is worth two where the grid fills the GPU several times (4096 rows of 5120 32.7 us, 34.7 with one), and with an
-  // edge, where registers let few threads onto an SM, from about one long row per SM on (4000 rows of 6387 54.9 us, 86.6
-  // with one; 160: 4.7, 6.2; but 100 of 5001 3.6, 3.1, and 400 of 1501 3.9, 3.3). The swiglu loses (12282 rows of 2048
+  // edge, where registers let few threads onto an SM, from about one long row per SM on (4000 rows of 6387 50.9 us, 80.6
+  // with one; 160: 4.5, 6.0; but 100 of 5001 3.4, 2.9, and 400 of 1501 3.7, 3.2). The swiglu loses (12282 rows of 2048
   // 24.2 us, 27.6 with two; 6000 of 2049 22.7, 26.0). A row keeps 32 threads.
   int nv = 1;
   while ((nchunk + nv - 1) / nv > 1024) nv *= 2;

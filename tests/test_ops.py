@@ -97,6 +97,19 @@ def test_rms_norm_quant_many_rows(ops, fmt, rows, n):
     check_quant(one.q, one.s, norm_ref(x[last], w, None)[1], fmt, 32 * U)
 
 
+@pytest.mark.parametrize("wdtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,n", [(3, 17), (9, 24), (40, 31), (301, 1501), (200, 2050), (150, 6387), (5, 8195)])
+def test_rms_norm_quant_odd_rows(ops, rows, n, dtype, wdtype):
+    """Every offset of a row to 16 bytes, one and two chunks a thread, weights of both types."""
+    x, r, w = rnd(126, rows, n, dtype=dtype), rnd(127, rows, n, dtype=dtype), (1 + 0.2 * rnd(128, n)).to(wdtype)
+    got = ops.rms_norm_quant(x, w, r, fmt="int8", normed=True)
+    h, v = norm_ref(x, w, r)
+    assert torch.equal(got.residual.double(), h)
+    within(got.normed, v, v.abs() * (32 * U + BF[dtype]))
+    check_quant(got.q, got.s, v, "int8", 32 * U)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rows", [1, 2, 34, 255])
 @pytest.mark.parametrize("n", [1, 2, 3, 5, 7, 9])
