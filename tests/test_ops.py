@@ -548,6 +548,45 @@ def test_empty_batches(ops):
     assert ops.swiglu_quant(torch.empty((0, 256), device="cuda"))[1].shape == (0,)
 
 
+def test_offsets_past_32_bits(ops):
+    """Tensors of more than 2^31 values: the last rows are those of a small call on the same rows."""
+    byt = lambda t: t.contiguous().view(torch.uint8)
+    rows, n = 132000, 16383
+    x = torch.zeros((rows, n), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = rnd(140, 3, n, dtype=torch.bfloat16)
+    w = 1 + 0.2 * rnd(141, n)
+    got, want = ops.rms_norm_quant(x, w, x, fmt="int8"), ops.rms_norm_quant(x[-3:].clone(), w, x[-3:].clone(), fmt="int8")
+    check_quant(got.q[-3:], got.s[-3:], norm_ref(x[-3:], w, x[-3:])[1], "int8", 32 * U)
+    assert torch.equal(got.residual[-3:], want.residual) and not got.q[:-3].any()
+    del got
+    half = x.view(-1)[:rows * n // 2 // 8191 * 8191 * 2].view(-1, 2 * 8191)
+    half[-1] = rnd(142, 2 * 8191, dtype=torch.bfloat16)
+    q, s = ops.swiglu_quant(half)
+    q1, s1 = ops.swiglu_quant(half[-1:].clone())
+    assert torch.equal(q[-1:], q1) and torch.equal(s[-1:], s1)
+    del q, s, half
+    x[-3:] = rnd(140, 3, n, dtype=torch.bfloat16)
+    idx = torch.zeros((rows, 1), dtype=torch.int64, device="cuda")
+    idx[-2] = 1  # the last row of all, the others in order
+    order = ops.sort_tokens(idx, 2)
+    xs = ops.dispatch_tokens(x, order)
+    assert torch.equal(xs[-1], x[-2]) and torch.equal(xs[-2], x[-1])
+    assert torch.equal(ops.combine_tokens(xs, order)[-3:], x[-3:])
+    dy = xs.clone().requires_grad_()
+    wt = torch.ones((rows, 1), device="cuda", requires_grad=True)
+    ops.combine_tokens(dy, order, wt).backward(x)
+    assert torch.equal(dy.grad[-2:], xs[-2:])
+    within(wt.grad[-3:, 0], (x[-3:].double() ** 2).sum(-1), (x[-3:].double() ** 2).sum(-1) * (n / 32 + 16) * U)
+    del x, xs, dy
+    m, k = 290000, 48
+    a, sa, b, sb = codes(143, m, k), scales(144, m), codes(145, 2, 8191, k), scales(146, 2, 8191)
+    out = ops.int8_gemm(a, sa, b[0], sb[0], out_dtype=torch.bfloat16)
+    assert torch.equal(byt(out[-5:]), byt(ops.int8_gemm(a[-5:], sa[-5:], b[0], sb[0], out_dtype=torch.bfloat16)))
+    off = torch.tensor([0, m - 7, m - 2], dtype=torch.int32, device="cuda")
+    ops.int8_grouped_gemm(a, sa, b, sb, off, out=out)
+    assert torch.equal(out[-7:-2], ops.int8_gemm(a[-7:-2], sa[-7:-2], b[1], sb[1], out_dtype=torch.bfloat16)) and not out[-2:].any()
+
+
 def test_refusals(ops):
     x, w = rnd(43, 4, 256, dtype=torch.bfloat16), torch.ones(256, device="cuda")
     for bad, err in ((lambda: ops.rms_norm_quant(x.half(), w), TypeError), (lambda: ops.rms_norm_quant(x, w[:128]), ValueError),
