@@ -134,7 +134,9 @@ DSMOE_API int dsmoe_act_quant(const void* x, int x_dtype, long long M, long long
 /* r = x + residual rounded to dtype (residual NULL: r = x), v = r / sqrt(mean(r^2) + eps) * weight per
  * row, v quantized: q_dtype DSMOE_DTYPE_E4M3 as in dsmoe_act_quant (one scale per 128 values, hidden a
  * multiple of 128, pow2 as there, s [rows, hidden / 128]), DSMOE_DTYPE_I8 with one scale per row,
- * s = max(amax, 1e-4) / 127, q = rint(v / s), s [rows]. residual_out (r; may be residual or x itself)
+ * s = max(amax, 1e-4) / 127, q = rint(v / s), s [rows]. Scales are rounded once (dsmoe_act_quant's for the
+ * same v); codes are v times the scale's fp32 reciprocal: beside a tie the other neighbour of v / s may come out.
+ * residual_out (r; may be residual or x itself)
  * and normed (v rounded to dtype) may be NULL. dtype F32 or BF16, weight [hidden] F32 or BF16, hidden
  * <= 16384. Squares are summed in fp32; a row with an infinity or NaN, or whose squares overflow, gets NaN
  * scales. Pointers other than s are 16-byte aligned.

@@ -258,11 +258,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-__device__ __forceinline__ float scale_of(float amax, float inv_top, int pow2) {
+// amax / top rounded once, as act_quant's: the same amax gives the same scale to the last bit. The product with the
+// reciprocal is a unit off for every second amax; what it leaves over, added, makes it the rounded quotient (division by
+// a divisor known in advance, Brisebarre, Muller and Raina 2004; compared with the division over all mantissas). A
+// division instruction sequence costs int8 rows of 2048 6 % (26.2, 27.7 us). inf and NaN come out as NaN.
+template <int TOP>
+__device__ __forceinline__ float scale_of(float amax, int pow2) {
+  constexpr float kInv = 1.0f / TOP;
   amax = amax < kAmaxFloor ? kAmaxFloor : amax;  // a NaN stays
-  float s = amax * inv_top;
+  const float p = amax * kInv;
+  float s = fmaf(fmaf(-p, (float)TOP, amax), kInv, p);
   if (pow2) {
-    s = amax / 448.0f;  // exact where it is a power of 2: the product with the reciprocal may lie above
     int e;
     const float m = frexpf(s, &e);
     if (s < INFINITY) s = ldexpf(1.0f, m == 0.5f ? e - 1 : e);
@@ -305,7 +311,9 @@ __device__ __forceinline__ void row_reduce(float& sum, float& top, int tpr) {
   if (MAX) top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < nw ? smax[w0 + lane] : 0u));
 }
 
-// v * mul to 8 bits with its scales; top: the row's max |v| (int8), mul: the row's factor that v still lacks.
+// v * mul to 8 bits with its scales; top: the row's max |v| (int8), mul: the row's factor that v still lacks. A code is
+// v * (mul * (1 / s)) rounded: one factor for all values instead of a division for each, which is within 6 * 2^-24 of
+// v mul / s, so that the code is its neighbour where the quotient lies that near to a tie (e4m3: 10 of 21 million codes).
 template <int VEC, int NV, bool FP8, bool EDGE>
 __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][VEC], float mul, float top, long long row,
                                             int t, bool live) {
@@ -320,7 +328,7 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
       // the 128 values of a block are 16 (bf16) or 32 (fp32) neighbouring lanes' chunks
 #pragma unroll
       for (int o = 64 / VEC; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float s = scale_of(m * fabsf(mul), 1.0f / 448.0f, a.pow2);
+      const float s = scale_of<448>(m * fabsf(mul), a.pow2);
       const float f = mul * __fdividef(1.0f, s);
       if (p.hi) {
         if (p.k % 128 == 0) a.s[row * (a.n / 128) + p.k / 128] = s;
@@ -334,7 +342,7 @@ __device__ __forceinline__ void quant_store(const Args& a, const float (&v)[NV][
       }
     }
   } else {
-    const float s = scale_of(top * fabsf(mul), 1.0f / 127.0f, 0);
+    const float s = scale_of<127>(top * fabsf(mul), 0);
     const float f = mul * __fdividef(1.0f, s);
     if (t == 0 && live) a.s[row] = s;
     const bool fine = s == s;  // else the row holds a NaN or an infinity: the code 0 throughout

@@ -49,7 +49,8 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, residual: Optional[tor
     ``int8_gemm``. ``normed``: also v in x's dtype (the router's input). ``inplace``: the new residual is
     written over ``residual``, which must be contiguous.
 
-    v is quantized from fp32. A row holding an infinity or NaN, or whose squares overflow fp32, has NaN scales."""
+    v is quantized from fp32; a scale is the quotient rounded once (``act_quant``'s, bit for bit, for the same v), a code
+    v times the scale's reciprocal, rounded: beside a tie it may be the other neighbour of v / s. A row holding an infinity or NaN, or whose squares overflow fp32, has NaN scales."""
     return NormQuant._make(_ops.rms_norm_quant(x, weight, residual, eps, fmt, scale_fmt is not None, bool(normed),
                                                bool(inplace)))
 

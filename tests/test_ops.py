@@ -785,3 +785,21 @@ def test_int8_experts_layer(ops):
     # beside the layer's own float formulas: int8 with one scale per row keeps the direction
     ref = torch.nn.functional.cosine_similarity(y.double(), want, dim=1)
     assert float(ref[torch.arange(P, device="cuda") != 7].min()) > 0.99
+
+
+@pytest.mark.parametrize("rows,n", [(4096, 512), (3, 5120), (65, 16384)])
+def test_scales_are_act_quants(ops, rows, n):
+    """The same rows, in fp32, through act_quant and through a division per row: the same scales, to the last bit."""
+    import kernel
+    x, w = rnd(130, rows, n, scale=3.0), 1 + 0.2 * rnd(131, n)
+    for scale_fmt in (None, "ue8m0"):
+        got = ops.rms_norm_quant(x, w, normed=True, scale_fmt=scale_fmt)
+        q, s = kernel.act_quant(got.normed, 128, scale_fmt)
+        assert torch.equal(got.s, s)
+        # codes: v times a reciprocal, within 8 u of the quotient: only values that near to a tie change sides. Ties lie
+        # at least 2^-4 of the value apart, so these are 16 u / 2^-4 = 2^-16 of all values (twice that, and a few)
+        other = q.view(torch.uint8) != got.q.view(torch.uint8)
+        assert int(other.sum()) <= 8 + 2.0 ** -15 * other.numel()
+    got = ops.rms_norm_quant(x, w, normed=True, fmt="int8")
+    top = got.normed.abs().amax(-1).clamp(min=1e-4)
+    assert torch.equal(got.s, torch.div(top, torch.full_like(top, 127.0)))
