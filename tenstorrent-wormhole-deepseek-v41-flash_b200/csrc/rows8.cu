@@ -11,9 +11,9 @@
 // max|r w|: since amax(v) = max|r w| / sqrt(..), both come out of one block reduction, so a row costs
 // one barrier. r is the rounded residual (what the next layer adds to), sums and products are fp32.
 // Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.6 us (5.8 TB/s; a copy of those bytes
-// 28.9), one row 2.3 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.2 us to e4m3 (5.2 TB/s; 19.3), 26.0 to int8:
+// 28.9), one row 2.4 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.4 us to e4m3 (5.2 TB/s; 19.3), 26.5 to int8:
 // about 22 instructions a value keep the issue slots two thirds busy. Rows that are not a multiple of 16 bytes cost
-// shifts and masks: swiglu of 6000 x 2049 to int8 22.7 us (2.7 TB/s), norm of 4000 x 6387 with residual 50.9 (3.5).
+// shifts and masks: swiglu of 6000 x 2049 to int8 22.4 us (2.7 TB/s), norm of 4000 x 6387 with residual 50.0 (3.6).
 // Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
 // or NaN or whose squares overflow fp32, and of a swiglu's row (e4m3: block) whose amax is not finite.
 #include "common.cuh"
@@ -492,39 +492,45 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
   return r;
 }
 
-// silu(g) u of two values, with g <= limit, |u| <= limit. exp(-g) = 2^t (1 + r) with t = -g log2(e) rounded and
-// r = -g - t ln 2, what the rounding lost, so the hardware's 2^t (2 units in the last place) and reciprocal (1) are all
-// that is approximated; the argument's own rounding would cost |g| units. exp's argument stops at 87, where silu(g) is
-// below 1e-35, so that the reciprocal stays a normal number. PACKED: both values in one instruction where it exists
-// (12282 rows of 2048: e4m3 24.2 us, 25.3 one by one; int8 rows without an edge are faster one by one, 26.0 and 27.7).
-template <bool PACKED>
+// silu(g) u of two values, with g <= limit, |u| <= limit, as (-g) (-u) / (1 + exp(-g)). exp(n) of n = -g is
+// 2^t (1 + r) with t = n log2(e) rounded and r = n - t ln 2, what the rounding lost, so the hardware's 2^t (2 units in the
+// last place) and reciprocal (1) are all that is approximated; the argument's own rounding would cost |g| units. t
+// stops at 87 log2(e), before 2^t overflows, but r does not: past it the sum grows on, and from n = 87.5 on (silu(g) above
+// -1e-36) its reciprocal is 0 and takes every finite gate to 0 and -inf to the formula's NaN. BIG: limits past 1e38, where t
+// needs a floor too; chosen at launch, as the two in one kernel take 29.4 us where one takes 24.4 (e4m3, 12282 x 2048).
+// PACKED: both values in one instruction where it exists (the same rows when this was chosen: e4m3 24.2 us, 25.3 one by
+// one; int8 rows without an edge are faster one by one, 26.0 and 27.7).
+template <bool PACKED, bool BIG>
 __device__ __forceinline__ void swiglu2(float& g0, float& g1, float u0, float u1, float limit) {
-  g0 = min_nan(g0, limit);
-  g1 = min_nan(g1, limit);
-  u0 = max_nan(min_nan(u0, limit), -limit);
-  u1 = max_nan(min_nan(u1, limit), -limit);
+  const float n0 = max_nan(-g0, -limit), n1 = max_nan(-g1, -limit);
+  u0 = max_nan(min_nan(-u0, limit), -limit);
+  u1 = max_nan(min_nan(-u1, limit), -limit);
   constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
-  const float a0 = min_nan(-g0, 87.0f), a1 = min_nan(-g1, 87.0f);
+  float a0 = min_nan(n0, 87.0f), a1 = min_nan(n1, 87.0f);
+  if (BIG) {
+    a0 = max_nan(a0, -200.0f);
+    a1 = max_nan(a1, -200.0f);
+  }
   float t0, t1, e0, e1;
   if constexpr (PACKED) {
-    const F2 a = f2(a0, a1), t = f2_mul(a, f2(kLog2e, kLog2e)), r = f2_fma(t, f2(-kLn2, -kLn2), a);
+    const F2 n = f2(n0, n1), t = f2_mul(f2(a0, a1), f2(kLog2e, kLog2e)), r = f2_fma(t, f2(-kLn2, -kLn2), n);
     f2_get(t, t0, t1);
     e0 = exp2_hw(t0);
     e1 = exp2_hw(t1);
     const F2 e = f2(e0, e1);
     f2_get(f2_add(f2_fma(e, r, e), f2(1.0f, 1.0f)), t0, t1);
-    f2_get(f2_mul(f2_mul(f2(g0, g1), f2(rcp_hw(t0), rcp_hw(t1))), f2(u0, u1)), g0, g1);
+    f2_get(f2_mul(f2_mul(n, f2(rcp_hw(t0), rcp_hw(t1))), f2(u0, u1)), g0, g1);
   } else {
     t0 = a0 * kLog2e;
     t1 = a1 * kLog2e;
     e0 = exp2_hw(t0);
     e1 = exp2_hw(t1);
-    g0 = g0 * rcp_hw(1.0f + fmaf(e0, fmaf(t0, -kLn2, a0), e0)) * u0;
-    g1 = g1 * rcp_hw(1.0f + fmaf(e1, fmaf(t1, -kLn2, a1), e1)) * u1;
+    g0 = n0 * rcp_hw(1.0f + fmaf(e0, fmaf(t0, -kLn2, n0), e0)) * u0;
+    g1 = n1 * rcp_hw(1.0f + fmaf(e1, fmaf(t1, -kLn2, n1), e1)) * u1;
   }
 }
 
-template <typename T, int NV, bool FP8, bool EDGE>
+template <typename T, int NV, bool FP8, bool EDGE, bool BIG>
 __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
   constexpr int VEC = 16 / sizeof(T);
   pdl_wait();
@@ -571,7 +577,7 @@ __global__ void __launch_bounds__(1024) swiglu_kernel(const Args a) {
     x[j].get(v[j]);
     y[j].get(u);
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) swiglu2<FP8 || EDGE>(v[j][i], v[j][i + 1], u[i], u[i + 1], a.limit);
+    for (int i = 0; i < VEC; i += 2) swiglu2<FP8 || EDGE, BIG>(v[j][i], v[j][i + 1], u[i], u[i + 1], a.limit);
     if (EDGE && (p.lo != 0 || p.hi != VEC)) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
@@ -595,7 +601,10 @@ int sm_count() {
 template <bool NORM, typename T, int NV, bool FP8, bool EDGE>
 void launch(const Args& a, cudaStream_t st) {
   const long long grid = (a.rows + a.rpc - 1) / a.rpc;
-  launch_pdl(NORM ? norm_kernel<T, NV, FP8, EDGE> : swiglu_kernel<T, NV, FP8, EDGE>, dim3((unsigned)grid), dim3(a.tpr, a.rpc), 0, st, a);
+  launch_pdl(NORM               ? norm_kernel<T, NV, FP8, EDGE>
+             : a.limit > 1e38f ? swiglu_kernel<T, NV, FP8, EDGE, true>
+                               : swiglu_kernel<T, NV, FP8, EDGE, false>,
+             dim3((unsigned)grid), dim3(a.tpr, a.rpc), 0, st, a);
 }
 template <bool NORM, typename T, bool FP8, bool EDGE>
 void launch_nv(const Args& a, int nv, cudaStream_t st) {

@@ -60,7 +60,8 @@ def swiglu_quant(gu: torch.Tensor, row_weight: Optional[torch.Tensor] = None, *,
     """(q, s) of silu(min(g, limit)) * clamp(u, -limit, limit) * row_weight for gu [..., 2 * inter] = g | u.
 
     The activation of ``Expert`` (dsv41/tt/moe.py:133-139) between two 8-bit products; formats and scales
-    as in ``rms_norm_quant``; a row (fp8: a block) whose amax is not finite has the scale NaN. ``row_weight``
+    as in ``rms_norm_quant``; a row (fp8: a block) whose amax is not finite has the scale NaN (a gate of -inf among them, as
+    silu(-inf) is NaN; every finite one down to the type's lowest value gives its silu, 0). ``row_weight``
     [...] fp32 (e.g. routing weights) is applied before the quantization."""
     return _ops.swiglu_quant(gu, row_weight, limit, fmt, scale_fmt is not None)
 

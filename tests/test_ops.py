@@ -803,3 +803,39 @@ def test_scales_are_act_quants(ops, rows, n):
     got = ops.rms_norm_quant(x, w, normed=True, fmt="int8")
     top = got.normed.abs().amax(-1).clamp(min=1e-4)
     assert torch.equal(got.s, torch.div(top, torch.full_like(top, 127.0)))
+
+
+FAR = [-87.25, -88.0, -89.0, -104.0, -1e4, -1e30, -1e32, -1e36]
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt,n", [("fp8", 256), ("int8", 256), ("int8", 257), ("int8", 1500), ("int8", 1501)])
+def test_swiglu_far_negative_gates(ops, fmt, n, dtype, weighted):
+    """Gates down to the type's lowest value (a masked channel) are 0, and leave their row's scale alone."""
+    far = FAR + [float(torch.finfo(dtype).min)]
+    gu = rnd(140, 3 * len(far), 2 * n, dtype=dtype)
+    gu[:, n:][:, ::7] = -10.0
+    wr = rnd(141, gu.shape[0]) * 40.0 if weighted else None
+    for i, g in enumerate(far):
+        gu[3 * i, 5] = g        # one channel among others
+        gu[3 * i + 1, :n] = g   # the whole row
+        gu[3 * i + 2, :n:3] = g
+    q, s = ops.swiglu_quant(gu, wr, fmt=fmt)
+    v = swiglu_ref(gu, wr)
+    # 17 roundings of the value; where the reciprocal of 1 + exp(-g) falls below fp32's normal range it is 0: 1e-36 u wr
+    check_quant(q, s, v, fmt, 17 * U)
+    assert not q[1::3].float().any() and bool((s[1::3] == torch.tensor(1e-4) / (448.0 if fmt == "fp8" else 127.0)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt,n", [("fp8", 128), ("int8", 128), ("int8", 129)])
+def test_swiglu_without_a_limit(ops, fmt, n, dtype):
+    gu = rnd(142, 4, 2 * n, dtype=dtype, scale=20.0)
+    top = float(torch.finfo(dtype).max)
+    gu[1, 3], gu[1, n + 3] = top, 0.25
+    gu[2, 3], gu[2, n + 3] = -top, top
+    gu[3, 3], gu[3, n + 3] = 2.0 ** 100, 2.0 ** 20
+    for limit in (float("inf"), top):
+        q, s = ops.swiglu_quant(gu, limit=limit, fmt=fmt)
+        check_quant(q, s, swiglu_ref(gu, None, limit), fmt, 16 * U)
