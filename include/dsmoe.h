@@ -166,6 +166,11 @@ DSMOE_API int dsmoe_int8_grouped_gemm(const int8_t* a, const float* a_s, long lo
                                       const float* b_s, int n_experts, long long N, const int* offsets, void* out,
                                       int out_dtype, void* stream);
 
+/* How long the int8 products of later calls (of this process) wait on the device for their operands to land before
+ * they give up and write NaN in place of the sums: 0..1000000000 ns, which is the default. With 0 they give up before the
+ * first: the failure path's test. */
+DSMOE_API int dsmoe_int8_operand_wait(long long ns);
+
 /* Choices sorted by (expert, token, choice): idx [P, k] int64 -> pos [P, k] int32 (row of each choice, -1
  * where idx is outside 0..n_experts-1: dropped), src [P k] int32 (choice t k + j of each row, -1 behind the
  * last), offsets [n_experts + 1] int32 (first row of each expert). k <= 64, n_experts <= 1024, P k < 2^30. */

@@ -20,7 +20,7 @@
 // 256 x 4096 x 5120 12.1. gemm_i8_pair_kernel, for many, is bound by the tensor pipe and, in a long run, by the power
 // limit: CTA pairs on 256 x 512 tiles, as the bytes an SM takes in hold back smaller tiles (4096 x 4096 x 5120: 128 x 256
 // by one CTA 98.6 us, 256 x 256 by a pair 69.3, 256 x 480 61.5, 2790 TOP/s; 70 us when it runs for 0.15 s).
-// Every wait is bounded; where one expired, the outputs are NaN.
+// Every wait is bounded; where one expired, the outputs are NaN: those of the whole cluster that shares the sums.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -50,6 +50,7 @@ struct Args {
   void* out;           // [M][N]
   int M, N, K, E, nkb, TT, BR, RS, NTN, out_f32;
   unsigned tcols;      // tensor memory columns (one-tile kernel)
+  uint64_t land_ns;    // how long the MMA issuer waits for a stage's operands; 0: it gives up before the first
 };
 
 
@@ -332,10 +333,14 @@ __global__ void __launch_bounds__(NT) gemm_i8_kernel(const __grid_constant__ Arg
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tslot;
-  auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
+  auto give_up = [&] {
+    *abortf = 1;
+    __threadfence_block();  // seen by whoever sees an arrival that follows
+  };
+  auto wait = [&](uint64_t* bar, uint32_t par, uint64_t limit_ns = kWaitNs) -> bool {
     if (*abortf) return false;
-    if (!mbar_wait(bar, par, kWaitNs)) {
-      *abortf = 1;
+    if (!mbar_wait(bar, par, limit_ns)) {
+      give_up();
       return false;
     }
     return true;
@@ -367,8 +372,9 @@ __global__ void __launch_bounds__(NT) gemm_i8_kernel(const __grid_constant__ Arg
                              ((uint32_t)(((t.cols + 15) >> 4) * 2) << 17);
       const uint64_t da0 = desc_sw128(smem_u32(ring)), db0 = desc_sw128(smem_u32(ring + TM * 128));
       Ring p;
+      if (!a.land_ns) give_up();
       for (int kb = kb0; kb < kb1; ++kb, p.next(a.RS)) {
-        if (!wait(&full[p.s], p.par)) break;
+        if (!wait(&full[p.s], p.par, a.land_ns)) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint64_t o = (uint64_t)(p.s * (SB >> 4));
 #pragma unroll
@@ -523,10 +529,14 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
   cluster_sync();  // both CTAs' barriers and tensor memory exist
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = *tslot;
-  auto wait = [&](uint64_t* bar, uint32_t par) -> bool {
+  auto give_up = [&] {
+    *abortf = 1;
+    __threadfence_block();  // seen by whoever sees an arrival that follows
+  };
+  auto wait = [&](uint64_t* bar, uint32_t par, uint64_t limit_ns = kWaitNs) -> bool {
     if (*abortf) return false;
-    if (!cluster_wait(bar, par, kWaitNs)) {
-      *abortf = 1;
+    if (!cluster_wait(bar, par, limit_ns)) {
+      give_up();
       return false;
     }
     return true;
@@ -564,8 +574,14 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
           for (int b = 0; b < nb1; ++b) tma_2d_pair(st + TM * 128 + 16384 + b * PBR * 128, &a.ta, kb * 128, y1 + b * PBR, bar);
         }
       }
-      // every copy issued has landed (its MMAs have read it) before the CTA may exit
-      for (int i = issued - 1; i >= 0 && i >= issued - a.RS; --i) cluster_wait(&empty[i % a.RS], (i / a.RS) & 1, kWaitNs);
+      // Every copy issued has landed before the pair may exit: both CTAs' report to the leader's barriers, and neither
+      // leaves without the other. The follower sees its own only through the MMAs that read them, of which an issuer
+      // that gave up runs none: then it waits out the limit, one for all stages.
+      const uint64_t t0 = globaltimer_ns();
+      for (int i = issued - 1; i >= 0 && i >= issued - a.RS; --i) {
+        const uint64_t spent = globaltimer_ns() - t0;
+        cluster_wait(rank == 0 ? &full[i % a.RS] : &empty[i % a.RS], (i / a.RS) & 1, spent < kWaitNs ? kWaitNs - spent : 0);
+      }
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -574,6 +590,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
       int slot = 0;  // halves of the tensor memory used so far
       Ring p;
       bool ok = true;
+      if (!a.land_ns) give_up();
       for (int tile = cid; tile < g.tiles && ok; tile += ncl) {
         const Tile t = locate(tile);
         const int w0 = width(t.cols, 0), w1 = width(t.cols, 1), n = w1 ? 2 : 1;
@@ -584,7 +601,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
         const uint32_t id0 = idesc0 | ((uint32_t)(w0 >> 3) << 17), id1 = idesc0 | ((uint32_t)(w1 >> 3) << 17);
         const uint32_t d0 = tmem + (uint32_t)((slot & 1) * 256), d1 = tmem + (uint32_t)(((slot + 1) & 1) * 256);
         for (int kb = 0; kb < a.nkb; ++kb, p.next(a.RS)) {
-          if (!wait(&full[p.s], p.par)) {
+          if (!wait(&full[p.s], p.par, a.land_ns)) {
             ok = false;
             break;
           }
@@ -599,6 +616,8 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
           }
           commit_pair(&empty[p.s]);
         }
+        // incomplete sums are not announced: the other CTA does not see this one's flag, its wait for them expires
+        if (!ok) break;
         for (int h = 0; h < n; ++h) commit_pair(&accf[(slot + h) & 1]);
         slot += n;
       }
@@ -645,6 +664,7 @@ __global__ void __launch_bounds__(NT, 1) gemm_i8_pair_kernel(const __grid_consta
 
 // ------------------------------------------------------------------ host side
 std::atomic<void*> g_encode{nullptr};
+std::atomic<unsigned long long> g_land_ns{kWaitNs};
 
 int encoder(PFN_cuTensorMapEncodeTiled_v12000* fn) {
   void* p = g_encode.load();
@@ -827,6 +847,7 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   a.nkb = (int)((K + 127) / 128);
   a.NTN = (int)((N + TM - 1) / TM);
   a.out_f32 = out_dtype == DSMOE_DTYPE_F32;
+  a.land_ns = g_land_ns.load(std::memory_order_relaxed);
   const size_t tables = 1024 + (2 * MAXRS + 9) * 8 + 16 + 2 * 256 * 4 + 48 + 2 * (E + 1) * 4 + 64;
   const Plan p = plan(M, N, a.nkb, offsets ? E : 0, sms, tables, optin);
   a.TT = p.TT;
@@ -877,6 +898,13 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
 }  // namespace dsmoe
 
 using namespace dsmoe;
+
+extern "C" int dsmoe_int8_operand_wait(long long ns) {
+  DSMOE_REQUIRE(ns >= 0 && ns <= (long long)gemm_i8::kWaitNs, DSMOE_ERR_ARG, "int8_operand_wait: %lld ns (0..%lld)", ns,
+                (long long)gemm_i8::kWaitNs);
+  gemm_i8::g_land_ns.store((unsigned long long)ns);
+  return DSMOE_OK;
+}
 
 extern "C" int dsmoe_int8_gemm(const int8_t* a, const float* a_s, long long M, long long K, const int8_t* b, const float* b_s,
                                long long N, void* out, int out_dtype, void* stream) {

@@ -56,6 +56,7 @@ _SIGS = {
     "dsmoe_swiglu_quant": ([_P, _I, _P, _LL, _LL, _F, _I, _I, _P, _P, _P], _I),
     "dsmoe_int8_gemm": ([_P, _P, _LL, _LL, _P, _P, _LL, _P, _I, _P], _I),
     "dsmoe_int8_grouped_gemm": ([_P, _P, _LL, _LL, _P, _P, _I, _LL, _P, _P, _I, _P], _I),
+    "dsmoe_int8_operand_wait": ([_LL], _I),
     "dsmoe_sort_tokens": ([_P, _LL, _I, _I, _P, _P, _P, _P], _I),
     "dsmoe_dispatch_rows": ([_P, _P, _P, _P, _I, _LL, _I, _LL, _P, _P, _P], _I),
     "dsmoe_combine_rows": ([_P, _I, _P, _P, _LL, _I, _LL, _P, _P], _I),

@@ -839,3 +839,39 @@ def test_swiglu_without_a_limit(ops, fmt, n, dtype):
     for limit in (float("inf"), top):
         q, s = ops.swiglu_quant(gu, limit=limit, fmt=fmt)
         check_quant(q, s, swiglu_ref(gu, None, limit), fmt, 16 * U)
+
+
+@pytest.fixture
+def operands_late():
+    """Int8 products whose operands count as late from the first on."""
+    from dsmoe import _lib as L
+    L.call("dsmoe_int8_operand_wait", 0)
+    yield
+    L.call("dsmoe_int8_operand_wait", 1000000000)
+
+
+# one-tile CTAs alone and in clusters of 2 to 8; pairs with fewer K blocks than ring stages, with more, several tiles each
+@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (8, 4096, 5120), (33, 64, 4096), (256, 1024, 2048), (4096, 512, 512),
+                                   (1024, 4096, 5120), (4096, 4096, 5120)])
+def test_int8_gemm_gives_nan_where_operands_are_late(ops, operands_late, m, n, k):
+    from dsmoe import _lib as L
+    a, b, sa, sb = codes(150, m, k), codes(151, n, k), scales(152, m), scales(153, n)
+    got = ops.int8_gemm(a, sa, b, sb, out_dtype=torch.float32)
+    torch.cuda.synchronize()
+    L.call("dsmoe_int8_operand_wait", 1000000000)
+    want = ops.int8_gemm(a, sa, b, sb, out_dtype=torch.float32)
+    within(want, (a.double() @ b.double().T) * sa.double()[:, None] * sb.double(), product_tol(want.double(), torch.float32))
+    assert bool(torch.isnan(got).all())  # both CTAs of a pair: neither stores the incomplete sums of the other's products
+
+
+def test_int8_grouped_gemm_gives_nan_where_operands_are_late(ops, operands_late):
+    from dsmoe import _lib as L
+    for counts, n, k in (([1] * 6, 256, 512), ([700, 0, 900, 1500], 512, 2048)):
+        m, e = sum(counts), len(counts)
+        a, b, sa, sb = codes(154, m, k), codes(155, e, n, k), scales(156, m), scales(157, e, n)
+        L.call("dsmoe_int8_operand_wait", 0)
+        got = ops.int8_grouped_gemm(a, sa, b, sb, group_offsets(counts), out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        L.call("dsmoe_int8_operand_wait", 1000000000)
+        want = ops.int8_grouped_gemm(a, sa, b, sb, group_offsets(counts), out_dtype=torch.float32)
+        assert bool(torch.isnan(got).all()) and not bool(torch.isnan(want).any())

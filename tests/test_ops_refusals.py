@@ -146,3 +146,8 @@ def test_quant_int8_channel():
     q, s = quant_int8_channel(w)
     assert q.dtype == torch.int8 and s.shape == (7,) and int(q.abs().max()) == 127 and not q[3].any()
     assert bool(((q.double() * s.double()[:, None] - w.double()).abs() <= s.double()[:, None] * (0.5 + 127 * 2.0 ** -22)).all())
+
+
+def test_int8_operand_wait_refuses():
+    assert _code("dsmoe_int8_operand_wait", -1) == -1 and _code("dsmoe_int8_operand_wait", 1000000001) == -1
+    assert _code("dsmoe_int8_operand_wait", 1000000000) == 0
