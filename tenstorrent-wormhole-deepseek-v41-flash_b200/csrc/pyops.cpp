@@ -98,8 +98,18 @@ int float_code(const char* name, const Tensor& t, const char* what) {
 Tensor empty(const Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
   return Tensor(at::detail::empty_cuda(shape, dtype, like.device(), std::nullopt));
 }
-// contiguous and 16-byte aligned; aligned: whether the kernel wants the alignment
+// Whether the memory does not hold the values: views that are conjugated or negated when they are read (or zeros
+// without memory), which are contiguous all the same.
+bool lazy(const Tensor& t) {
+  return t.key_set().has_any(
+      c10::DispatchKeySet({c10::DispatchKey::Conjugate, c10::DispatchKey::Negative, c10::DispatchKey::ZeroTensor}));
+}
+// contiguous, its values in memory and 16-byte aligned; aligned: whether the kernel wants the alignment
 Tensor dense(const Tensor& t, bool aligned = true) {
+  if (lazy(t)) {
+    const Tensor r = t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_conj().resolve_neg();
+    return r.is_contiguous() ? r : r.contiguous();
+  }
   Tensor c = t.is_contiguous() ? t : t.contiguous();
   return aligned && reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
 }
@@ -190,7 +200,8 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t h = x0.size(-1);
     want(name, w0, "weight", w0.scalar_type(), {h});
     if (r0.defined()) want(name, r0, "residual", x0.scalar_type(), x0.sizes());
-    value_check(!inplace || (r0.defined() && r0.is_contiguous()), name, "inplace needs a contiguous residual");
+    value_check(!inplace || (r0.defined() && r0.is_contiguous() && !lazy(r0)), name,
+                "inplace needs a contiguous residual that is no conjugate or negative view");
     Tensor q, s, out, y;
     const int code = quant_out(name, args[4], pow2, x0, h, q, s);
     const Tensor x = dense(x0), w = dense(w0), r = r0.defined() ? dense(r0) : r0;
@@ -272,8 +283,8 @@ PyObject* int8_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (out.defined()) {
       type_check(args[5] == Py_None || dt == out.scalar_type(), name, "out is ", out.scalar_type(), ", out_dtype ", dt);
       dt = out.scalar_type();
-      value_check(out.sizes() == at::IntArrayRef(shape) && out.is_contiguous(), name, "out must be a contiguous ",
-                  at::IntArrayRef(shape), " tensor");
+      value_check(out.sizes() == at::IntArrayRef(shape) && out.is_contiguous() && !lazy(out), name, "out must be a contiguous ",
+                  at::IntArrayRef(shape), " tensor and no conjugate or negative view");
     }
     type_check(dt == at::kFloat || dt == at::kBFloat16, name, "output dtype must be bfloat16 or float32, got ", dt);
     if (!out.defined()) out = empty(a0, shape, dt);
@@ -323,7 +334,7 @@ PyObject* sort_tokens(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 void check_order(const char* name, const Tensor& pos, const Tensor& off) {
   value_check(pos.scalar_type() == at::kInt && off.scalar_type() == at::kInt && pos.dim() == 2 && off.dim() == 1 &&
-                  pos.is_contiguous() && off.is_contiguous() && pos.size(1) >= 1 && pos.size(1) <= kMaxTopk &&
+                  pos.is_contiguous() && off.is_contiguous() && !lazy(pos) && !lazy(off) && pos.size(1) >= 1 && pos.size(1) <= kMaxTopk &&
                   off.size(0) >= 2 && off.size(0) <= kMaxExperts + 1,
               name, "order must come from sort_tokens");
 }

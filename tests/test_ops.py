@@ -875,3 +875,51 @@ def test_int8_grouped_gemm_gives_nan_where_operands_are_late(ops, operands_late)
         L.call("dsmoe_int8_operand_wait", 1000000000)
         want = ops.int8_grouped_gemm(a, sa, b, sb, group_offsets(counts), out_dtype=torch.float32)
         assert bool(torch.isnan(got).all()) and not bool(torch.isnan(want).any())
+
+
+@pytest.mark.parametrize("dtype", [torch.complex64, torch.complex128])
+def test_dispatch_of_conjugates(ops, dtype):
+    g = torch.Generator().manual_seed(160)
+    z = torch.randn((5, 24), generator=g, dtype=dtype).to("cuda")
+    order = ops.sort_tokens(torch.tensor([[1, 0], [2, -1], [0, 1], [1, 2], [0, 2]], device="cuda"), 3)
+    for x in (z.conj(), z.conj()[:, 1:], z.conj().imag, z):
+        want = torch.zeros((10, x.shape[1]), dtype=x.dtype, device="cuda")
+        for t in range(5):
+            for j in range(2):
+                if order.pos[t, j] >= 0:
+                    want[order.pos[t, j]] = x[t].resolve_conj()
+        got = ops.dispatch_tokens(x, order)
+        assert not got.is_conj() and not got.is_neg() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_negative_views(ops, dtype):
+    """Views that are negated when they are read: as inputs like any other tensor, refused where a kernel would write them."""
+    neg = torch._neg_view
+    x, r, w, gu = rnd(161, 6, 256, dtype=dtype), rnd(162, 6, 256, dtype=dtype), rnd(163, 256), rnd(164, 6, 512, dtype=dtype)
+    wr, flat = rnd(165, 6), torch.cat([x.new_zeros(1), x.flatten()])[1:].view(6, 256)
+    bits = lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+    same = lambda a, b: all((p is None and q is None) or torch.equal(bits(p), bits(q)) for p, q in zip(a, b))
+    for fmt in ("fp8", "int8"):
+        assert same(ops.rms_norm_quant(neg(x), neg(w), neg(r), fmt=fmt), ops.rms_norm_quant(-x, -w, -r, fmt=fmt))
+        assert same(ops.rms_norm_quant(neg(flat), w, fmt=fmt), ops.rms_norm_quant(-x, w, fmt=fmt))
+        assert same(ops.swiglu_quant(neg(gu), neg(wr), fmt=fmt), ops.swiglu_quant(-gu, -wr, fmt=fmt))
+    a, b, sa, sb = codes(166, 6, 256), codes(167, 2, 512, 256), scales(168, 6), scales(169, 2, 512)
+    off = group_offsets([2, 4])
+    assert torch.equal(ops.int8_gemm(a, neg(sa), b[0], neg(sb[0])), ops.int8_gemm(a, sa, b[0], sb[0]))
+    assert torch.equal(ops.int8_grouped_gemm(a, neg(sa), b, sb, off), ops.int8_grouped_gemm(a, -sa, b, sb, off))
+    idx = torch.tensor([[0, 1], [2, -1], [1, 0]], device="cuda")
+    assert same(ops.sort_tokens(neg(-idx), 3), ops.sort_tokens(idx, 3))
+    order, wt = ops.sort_tokens(idx, 3), rnd(170, 3, 2)
+    leaves = [t.clone().requires_grad_() for t in (x, wt)]
+    y, want = ops.combine_tokens(neg(leaves[0]), order, neg(leaves[1])), ops.combine_tokens(-x, order, -wt)
+    assert torch.equal(y, want)
+    dy = rnd(171, 3, 256, dtype=dtype)
+    got = torch.autograd.grad(y, leaves, neg(dy))
+    leaves = [t.clone().requires_grad_() for t in (x, wt)]
+    assert same(got, torch.autograd.grad(ops.combine_tokens(-leaves[0], order, -leaves[1]), leaves, -dy))
+    for call in (lambda: ops.rms_norm_quant(x, w, neg(r), inplace=True),
+                 lambda: ops.int8_gemm(a, sa, b[0], sb[0], out=neg(torch.zeros(6, 512, device="cuda", dtype=dtype))),
+                 lambda: ops.combine_tokens(x, order._replace(pos=neg(order.pos)))):
+        with pytest.raises(ValueError, match="negative view|must come from sort_tokens"):
+            call()
