@@ -17,6 +17,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/core/DefaultDtype.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -70,8 +71,12 @@ const Tensor& tensor(const char* name, PyObject* o) {
 // None -> an undefined tensor
 Tensor maybe(const char* name, PyObject* o) { return o == Py_None ? Tensor() : tensor(name, o); }
 
+// All on one GPU, and none with a forward-mode tangent, which a kernel would lose without a word.
 void same_device(const char* name, std::initializer_list<const Tensor*> ts) {
   const Tensor& a = **ts.begin();
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const Tensor* t : ts)
+      value_check(!t->defined() || !t->_fw_grad(0).defined(), name, "has no forward-mode derivative: pass primals without tangents");
   for (const Tensor* t : ts) {
     if (!t->defined()) continue;
     value_check(t->is_cuda(), name, "dsmoe kernels take CUDA tensors only, got ", t->sizes(), " on ", t->device());

@@ -13,7 +13,8 @@ its kernels:
 
 CUDA tensors only, on the tensors' device and that device's current stream; every call can be captured into a CUDA graph and
 none keeps anything between calls. Inputs that are not contiguous are copied. The 8-bit operators
-have no gradient and refuse tensors that require one. Checks, allocations and the C ABI call of each
+have no gradient and refuse tensors that require one; none has a forward-mode derivative, and all refuse tensors that
+carry a tangent. Checks, allocations and the C ABI call of each
 operator are native (csrc/pyops.cpp, module ``dsmoe._ops``): there is no fallback if it is missing.
 """
 from typing import NamedTuple, Optional

@@ -923,3 +923,25 @@ def test_negative_views(ops, dtype):
                  lambda: ops.combine_tokens(x, order._replace(pos=neg(order.pos)))):
         with pytest.raises(ValueError, match="negative view|must come from sort_tokens"):
             call()
+
+
+def test_tensors_with_a_tangent_are_refused(ops):
+    from torch.autograd import forward_ad as fwd
+    x, w = torch.ones(2, 128).to("cuda"), torch.ones(128).to("cuda")
+    q, s = torch.ones(2, 128, dtype=torch.int8).to("cuda"), torch.ones(2).to("cuda")
+    order = ops.TokenOrder(torch.tensor([[0], [1]], dtype=torch.int32).to("cuda"), torch.tensor([0, 1], dtype=torch.int32).to("cuda"),
+                           torch.tensor([0, 1, 2], dtype=torch.int32).to("cuda"))
+    with fwd.dual_level():
+        d = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rms_norm_quant(d(x), w), lambda: ops.rms_norm_quant(x, d(w)),
+                     lambda: ops.rms_norm_quant(x, w, d(x)), lambda: ops.swiglu_quant(d(x)), lambda: ops.swiglu_quant(x, d(s)),
+                     lambda: ops.int8_gemm(q, d(s), q, s), lambda: ops.int8_gemm(q, s, q, d(s)),
+                     lambda: ops.int8_grouped_gemm(q, d(s), q[None], s[None], order.offsets[:2]),
+                     lambda: ops.dispatch_tokens(d(x), order), lambda: ops.dispatch_tokens(x, order, d(s)),
+                     lambda: ops.dispatch_tokens(d(x.clone().requires_grad_()), order),
+                     lambda: ops.combine_tokens(d(x), order), lambda: ops.combine_tokens(x, order, d(s[:, None]))):
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
+        assert torch.equal(ops.dispatch_tokens(fwd.unpack_dual(d(x)).primal, order), x)

@@ -151,3 +151,23 @@ def test_quant_int8_channel():
 def test_int8_operand_wait_refuses():
     assert _code("dsmoe_int8_operand_wait", -1) == -1 and _code("dsmoe_int8_operand_wait", 1000000001) == -1
     assert _code("dsmoe_int8_operand_wait", 1000000000) == 0
+
+
+def test_tensors_with_a_tangent_are_refused():
+    import dsmoe as ops
+    from torch.autograd import forward_ad as fwd
+    x, w = torch.ones(2, 128), torch.ones(128)
+    q, s = torch.ones(2, 128, dtype=torch.int8), torch.ones(2)
+    order = ops.TokenOrder(torch.tensor([[0], [1]], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32),
+                           torch.tensor([0, 1, 2], dtype=torch.int32))
+    with fwd.dual_level():
+        d = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.rms_norm_quant(d(x), w), lambda: ops.rms_norm_quant(x, d(w)),
+                     lambda: ops.rms_norm_quant(x, w, d(x)), lambda: ops.swiglu_quant(d(x)), lambda: ops.swiglu_quant(x, d(s)),
+                     lambda: ops.int8_gemm(q, d(s), q, s), lambda: ops.int8_gemm(q, s, q, d(s)),
+                     lambda: ops.int8_grouped_gemm(q, d(s), q[None], s[None], order.offsets[:2]),
+                     lambda: ops.dispatch_tokens(d(x), order), lambda: ops.dispatch_tokens(x, order, d(s)),
+                     lambda: ops.dispatch_tokens(d(x.clone().requires_grad_()), order),
+                     lambda: ops.combine_tokens(d(x), order), lambda: ops.combine_tokens(x, order, d(s[:, None]))):
+            with pytest.raises(ValueError, match="no forward-mode derivative"):
+                call()
