@@ -361,17 +361,39 @@ class Int8Experts:
         self.w2 = torch.zeros((n_experts, hidden, inter), dtype=torch.int8, device=self.device)
         self.s2 = torch.zeros((n_experts, hidden), dtype=torch.float32, device=self.device)
 
+    # the types whose bytes are the codes and the scales of a format
+    _CODES = {"fp8": (torch.uint8, torch.int8, torch.float8_e4m3fn), "fp4": (torch.uint8, torch.int8)}
+    _SCALES = {"fp8": (torch.float32,), "fp4": (torch.uint8, torch.int8, torch.float8_e8m0fnu)}
+
+    @classmethod
+    def _check_matrix(cls, fmt, name, q, s, n, k):
+        """The dequant kernels compute addresses from n and k alone, so what they read has to be there."""
+        if fmt not in cls._CODES:
+            raise ValueError(f"expert format {fmt!r}, expected one of {sorted(cls._CODES)}")
+        if fmt == "fp4" and k % 32:
+            raise ValueError(f"w{name}: FP4 needs rows of a multiple of 32 values, got {k}")
+        if q.dtype not in cls._CODES[fmt] or s.dtype not in cls._SCALES[fmt]:
+            raise TypeError(f"w{name} ({fmt}): codes of type {q.dtype} with scales of type {s.dtype}, expected one of "
+                            f"{cls._CODES[fmt]} with one of {cls._SCALES[fmt]}")
+        want = ((n, k), (-(-n // 128), -(-k // 128))) if fmt == "fp8" else ((n, k // 2), (n, k // 32))
+        if (tuple(q.shape), tuple(s.shape)) != want:
+            raise ValueError(f"w{name} ({fmt}): codes {tuple(q.shape)} with scales {tuple(s.shape)}, expected {want[0]} with "
+                             f"{want[1]}")
+
     def load_expert(self, e: int, ew: ExpertWeights) -> None:
-        """Requantize expert ``e`` from its checkpoint format (FP8 or FP4) to int8, on the GPU."""
+        """Requantize expert ``e`` from its checkpoint format (FP8 or FP4) to int8, on the GPU.
+
+        FP8: e4m3 codes [N, K] with fp32 scales [ceil(N / 128), ceil(K / 128)]; FP4: packed e2m1 [N, K / 2] with e8m0
+        scales [N, K / 32], K a multiple of 32. Other shapes and types are refused."""
         if not 0 <= e < self.n_experts:
             raise IndexError(e)
         i, h = self.inter, self.hidden
+        for m, n, k in (("1", i, h), ("3", i, h), ("2", h, i)):
+            self._check_matrix(ew.fmt, m, getattr(ew, "w" + m), getattr(ew, "s" + m), n, k)
         for q, s, n, k, dst, scale in ((ew.w1, ew.s1, i, h, self.w13[e, :i], self.s13[e, :i]),
                                        (ew.w3, ew.s3, i, h, self.w13[e, i:], self.s13[e, i:]),
                                        (ew.w2, ew.s2, h, i, self.w2[e], self.s2[e])):
             q, s = q.to(self.device).contiguous(), s.to(self.device).contiguous()
-            if tuple(q.shape) != (n, k if ew.fmt == "fp8" else k // 2):
-                raise ValueError(f"expert weights {tuple(q.shape)} do not match hidden {h} / inter {i} ({ew.fmt})")
             w = torch.empty((n, k), dtype=torch.float32, device=self.device)
             with torch.cuda.device(self.device):
                 if ew.fmt == "fp8":

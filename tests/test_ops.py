@@ -945,3 +945,17 @@ def test_tensors_with_a_tangent_are_refused(ops):
             with torch.no_grad(), pytest.raises(ValueError, match="no forward-mode derivative"):
                 call()
         assert torch.equal(ops.dispatch_tokens(fwd.unpack_dual(d(x)).primal, order), x)
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_int8_experts_take_the_formats_types(ops, fmt):
+    """Codes and scales as raw bytes or in their own types, from the CPU or the GPU: the same weights."""
+    h, i = 288, 160
+    ew = ops.make_expert(fmt, h, i, torch.Generator().manual_seed(1))
+    typed = {n: t.view(torch.float8_e4m3fn) if fmt == "fp8" and n[0] == "w" else
+             t.view(torch.float8_e8m0fnu) if fmt == "fp4" and n[0] == "s" else t for n, t in vars(ew).items() if n != "fmt"}
+    layer = ops.Int8Experts(h, i, 3)
+    for e, w in enumerate((ew, ops.ExpertWeights(fmt, **typed), ew.to("cuda"))):
+        layer.load_expert(e, w)
+    for t in (layer.w13, layer.s13, layer.w2, layer.s2):
+        assert bool(t[0].any()) and torch.equal(t[0], t[1]) and torch.equal(t[0], t[2])

@@ -171,3 +171,30 @@ def test_tensors_with_a_tangent_are_refused():
                      lambda: ops.combine_tokens(d(x), order), lambda: ops.combine_tokens(x, order, d(s[:, None]))):
             with pytest.raises(ValueError, match="no forward-mode derivative"):
                 call()
+
+
+@pytest.mark.parametrize("fmt", ["fp8", "fp4"])
+def test_int8_experts_refuse_weights_that_are_not_there(fmt):
+    """Codes and scales whose shape or type is not the format's never reach a kernel (none runs here: no GPU is needed)."""
+    import dsmoe
+    h, i = 288, 160
+    ew = dsmoe.make_expert(fmt, h, i, torch.Generator().manual_seed(0))
+    layer = dsmoe.Int8Experts(h, i, 2, device="cpu")
+    layer.w13.fill_(1)
+    short = {"s1": ew.s1[:-1], "s3": ew.s3[:, :-1], "s2": ew.s2.flatten(), "w1": ew.w1[:-1], "w2": ew.w2[:, :-16], "w3": ew.w3[None]}
+    wrong = {"s1": ew.s1.to(torch.float64), "s3": ew.s3.to(torch.bfloat16), "s2": ew.s2.to(torch.int32), "w1": ew.w1.to(torch.int16),
+             "w2": ew.w2.float()}
+    wrong["s3"] = ew.s3.to(torch.uint8) if fmt == "fp8" else ew.s3.float()  # the other format's type
+    for error, changes in ((ValueError, short), (TypeError, wrong)):
+        for name, value in changes.items():
+            with pytest.raises(error, match="codes"):
+                layer.load_expert(0, dsmoe.ExpertWeights(**{**vars(ew), name: value}))
+    with pytest.raises(ValueError, match="expert format"):
+        layer.load_expert(0, dsmoe.ExpertWeights(**{**vars(ew), "fmt": "int4"}))
+    with pytest.raises(IndexError):
+        layer.load_expert(2, ew)
+    if fmt == "fp4":  # hidden and inter in steps of 16 are the layer's; FP4 comes in groups of 32
+        odd = dsmoe.Int8Experts(304, i, 1, device="cpu")
+        with pytest.raises(ValueError, match="multiple of 32"):
+            odd.load_expert(0, ew)
+    assert bool((layer.w13 == 1).all())
