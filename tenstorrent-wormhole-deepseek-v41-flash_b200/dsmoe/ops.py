@@ -15,16 +15,33 @@ CUDA tensors only, on the tensors' device and that device's current stream; ever
 none keeps anything between calls. Inputs that are not contiguous are copied. The 8-bit operators
 have no gradient and refuse tensors that require one; none has a forward-mode derivative, and all refuse tensors that
 carry a tangent. Checks, allocations and the C ABI call of each
-operator are native (csrc/pyops.cpp, module ``dsmoe._ops``): there is no fallback if it is missing.
+operator are native (csrc/pyops.cpp, module ``dsmoe._ops``): there is no fallback if it is missing. It is
+built for one PyTorch and loaded by the first call, so the rest of the package does not need it.
 """
+import importlib
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib as L
-from . import _ops
 
-_ops.set_error_type(L.DsmoeError)
+
+class _Native:
+    """Stands in for the module until the first operator is called."""
+
+    def __getattr__(self, name):
+        global _ops
+        try:
+            native = importlib.import_module("._ops", __package__)
+        except ImportError as e:
+            raise ImportError(f"dsmoe.ops needs dsmoe/_ops.so, built for this PyTorch ({torch.__version__}): run make in csrc "
+                              f"({e})") from e
+        native.set_error_type(L.DsmoeError)
+        _ops = native
+        return getattr(native, name)
+
+
+_ops = _Native()
 
 
 class NormQuant(NamedTuple):
