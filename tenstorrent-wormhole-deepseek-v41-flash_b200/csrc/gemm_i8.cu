@@ -852,6 +852,8 @@ int run(const char* name, const int8_t* x, const float* a_s, long long M, long l
   const Plan p = plan(M, N, a.nkb, offsets ? E : 0, sms, tables, optin);
   a.TT = p.TT;
   a.BR = p.pair ? PBR : offsets ? std::min(p.TT, 64) : p.TT;
+  // a one-tile stage holds TT token rows, which its loads fill exactly: a last one in part would write into the next stage
+  DSMOE_REQUIRE(p.pair || a.TT % a.BR == 0, DSMOE_ERR_UNSUPPORTED, "%s: tile of %d tokens in loads of %d", name, a.TT, a.BR);
   a.NTN = (int)((N + (p.pair ? 2 : 1) * TM - 1) / ((p.pair ? 2 : 1) * TM));
   const long long tiles = a.NTN * (M / a.TT + (offsets ? std::min<long long>(E, M) : M % a.TT != 0));  // at most
   DSMOE_REQUIRE(tiles * p.S < (1LL << 31), DSMOE_ERR_ARG, "%s: too many tiles", name);
