@@ -31,6 +31,8 @@ class _Native:
 
     def __getattr__(self, name):
         global _ops
+        if name.startswith("__"):  # whoever looks at objects in general
+            raise AttributeError(name)
         try:
             native = importlib.import_module("._ops", __package__)
         except ImportError as e:

@@ -14,6 +14,7 @@ USE = """
 import dsmoe, kernel, torch
 from dsmoe import MoE, Expert, Int8Experts, ExpertStore, _lib
 assert kernel.int8_gemm is dsmoe.int8_gemm and _lib.lib.dsmoe_version() > 0
+assert not hasattr(dsmoe.ops._ops, "__wrapped__")
 for call in (lambda: dsmoe.sort_tokens(torch.zeros(2, 1, dtype=torch.int64), 2), lambda: kernel.swiglu_quant(torch.zeros(2, 4))):
     try:
         call()
@@ -51,7 +52,7 @@ def test_make_follows_pytorch(tmp_path):
         f.write_text("")
     cc = _script(tmp_path / "cc", 'while [ $# -gt 0 ]; do if [ "$1" = -o ]; then touch "$2"; echo "$2" >> "%s/log"; fi; shift; done\n'
                  % tmp_path)
-    py = _script(tmp_path / "py", 'case "$2" in *metadata*) [ -n "$FAKE_TORCH" ] && echo "$FAKE_TORCH" || exit 1;; *) echo /nowhere;; esac\n')
+    py = _script(tmp_path / "py", 'case "$2" in *cache_tag*) [ -n "$FAKE_TORCH" ] && echo "$FAKE_TORCH" || exit 1;; *) echo /nowhere;; esac\n')
 
     def make(torch):
         (tmp_path / "log").write_text("")
