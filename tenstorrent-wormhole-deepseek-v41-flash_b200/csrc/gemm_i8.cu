@@ -16,8 +16,8 @@
 // Two kernels. gemm_i8_kernel, for few tokens, is bound by the weights' bytes and by its own latencies: a cluster of up
 // to 8 CTAs shares a tile's K blocks and adds the integer partial sums through distributed shared memory (exact, so the
 // order does not matter); no workspace, nothing shared between calls. Set-up, first load, barrier and sum are about
-// 3.5 us of a call: 8 x 4096 x 5120 takes 6.4 to 7.0 us (3.2 of them the bytes at copy rate), 64 x 4096 x 5120 8.1,
-// 256 x 4096 x 5120 12.1. gemm_i8_pair_kernel, for many, is bound by the tensor pipe and, in a long run, by the power
+// 3.5 us of a call: 8 x 4096 x 5120 takes 7.9 us with weights from memory and 7.3 where three sets of them take turns
+// (3.2 are the bytes at copy rate), 64 x 4096 x 5120 9.0, 256 x 4096 x 5120 12.7, 512 x 4096 x 5120 16.2. gemm_i8_pair_kernel, for many, is bound by the tensor pipe and, in a long run, by the power
 // limit: CTA pairs on 256 x 512 tiles, as the bytes an SM takes in hold back smaller tiles (4096 x 4096 x 5120: 128 x 256
 // by one CTA 98.6 us, 256 x 256 by a pair 69.3, 256 x 480 61.5, 2790 TOP/s; 70 us when it runs for 0.15 s).
 // Every wait is bounded; where one expired, the outputs are NaN: those of the whole cluster that shares the sums.

@@ -1043,7 +1043,8 @@ __global__ void __launch_bounds__(FT, 1) moe_fused_kernel(FusedArgs a) {
   refill();  // router rows stream in while the token rows arrive
   // Past this point the previous kernel of the stream has completed and its writes are visible:
   // this call's tokens (often that kernel's output), the workspace, the exchange epoch. The next
-  // kernel may be scheduled now; it cannot be resident on an SM before this grid's CTA there exits.
+  // kernel may be scheduled now, beside this grid's CTAs where it is small enough; it waits for this
+  // grid to end before it touches memory. All CTAs of this grid are resident by then.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {

@@ -10,8 +10,8 @@
 // stays in registers between. The norm needs two values of the whole row, sum(r^2) and (int8)
 // max|r w|: since amax(v) = max|r w| / sqrt(..), both come out of one block reduction, so a row costs
 // one barrier. r is the rounded residual (what the next layer adds to), sums and products are fp32.
-// Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.6 us (5.8 TB/s; a copy of those bytes
-// 28.9), one row 2.4 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.4 us to e4m3 (5.2 TB/s; 19.3), 26.5 to int8:
+// Measured: 4096 rows of 5120 bf16 with residual, codes, scales and normed rows 32.7 us (5.8 TB/s; a copy of those bytes
+// 28.9), one row 2.4 to 2.6 us (a launch); swiglu of 12282 rows of 2 x 2048 bf16 24.4 us to e4m3 (5.2 TB/s; 19.3), 26.5 to int8:
 // about 22 instructions a value keep the issue slots two thirds busy. Rows that are not a multiple of 16 bytes cost
 // shifts and masks: swiglu of 6000 x 2049 to int8 22.4 us (2.7 TB/s), norm of 4000 x 6387 with residual 50.0 (3.6).
 // Scales that are not finite are NaN, so that the values read back as NaN: those of a norm's row that holds an infinity
