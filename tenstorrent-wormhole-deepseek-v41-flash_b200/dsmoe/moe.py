@@ -362,7 +362,7 @@ class Int8Experts:
         self.s2 = torch.zeros((n_experts, hidden), dtype=torch.float32, device=self.device)
 
     # the types whose bytes are the codes and the scales of a format
-    _CODES = {"fp8": (torch.uint8, torch.int8, torch.float8_e4m3fn), "fp4": (torch.uint8, torch.int8)}
+    _CODES = {"fp8": (torch.uint8, torch.int8, torch.float8_e4m3fn), "fp4": (torch.uint8, torch.int8, torch.float4_e2m1fn_x2)}
     _SCALES = {"fp8": (torch.float32,), "fp4": (torch.uint8, torch.int8, torch.float8_e8m0fnu)}
 
     @classmethod

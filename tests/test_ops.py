@@ -959,3 +959,14 @@ def test_int8_experts_take_the_formats_types(ops, fmt):
         layer.load_expert(e, w)
     for t in (layer.w13, layer.s13, layer.w2, layer.s2):
         assert bool(t[0].any()) and torch.equal(t[0], t[1]) and torch.equal(t[0], t[2])
+
+
+def test_int8_experts_take_packed_e2m1_in_its_own_type(ops):
+    h, i = 288, 160
+    ew = ops.make_expert("fp4", h, i, torch.Generator().manual_seed(2))
+    own = {n: t.view(torch.float4_e2m1fn_x2) if n[0] == "w" else t for n, t in vars(ew).items() if n != "fmt"}
+    layer = ops.Int8Experts(h, i, 2)
+    layer.load_expert(0, ew)
+    layer.load_expert(1, ops.ExpertWeights("fp4", **own))
+    for t in (layer.w13, layer.s13, layer.w2, layer.s2):
+        assert bool(t[0].any()) and torch.equal(t[0], t[1])
